@@ -216,6 +216,66 @@ int w4a16_linear_fused(uint16_t* y, const w4a16_weights_t* w, const uint16_t* x,
 int w4a16_repack_into_swiglu(const w4a16_weights_t* w, int dst_row_offset, const uint32_t* packed,
                              const uint16_t* scale, const uint32_t* zp, int out_f, int inter, void* stream);
 
+/* A linear layer with bias, activation and residual in its epilogue, for any number of tokens (one token, a verify block, a
+ * prompt):  y[m] = act(W x[m] + bias) + residual[m],  x bf16 [M][in_f], y and residual bf16 [M][out_f].
+ *   bias        bf16 [out_f] or NULL
+ *   activation  one of the codes below. GELU is the exact one (erf), GELU_TANH the tanh form. SWIGLU wants a container whose rows
+ *               were interleaved by w4a16_repack_into_swiglu, out_f a multiple of 32, and halves the row:
+ *               y, residual [M][out_f / 2], y = silu(gate) * up; the bias is [gate | up], in the checkpoint's order.
+ *   residual    or NULL; it may be y itself (updated in place), else it must not overlap y.
+ * The weights multiplied are those that w4a16_dequant_rows returns, whatever M is; sums, bias, activation and residual are
+ * fp32, rounded to bf16 once. (w4a16_linear_fused, for M <= 16, multiplies (q - z) s unrounded and rounds between the steps as the
+ * reference's separate kernels do.) No scratch; y must not overlap x or bias; x, y and residual 16-byte aligned. M = 0 does
+ * nothing. Rows are independent; the order of a row's sum over k, and so its last bits, goes by M and the layer's sizes. No
+ * reference counterpart (its elementwise kernels: src/kernels/elementwise.cu:35-49). */
+#define W4A16_ACT_NONE 0
+#define W4A16_ACT_SILU 1
+#define W4A16_ACT_GELU 2
+#define W4A16_ACT_GELU_TANH 3
+#define W4A16_ACT_SWIGLU 4
+int w4a16_linear_epilogue(uint16_t* y, const w4a16_weights_t* w, const uint16_t* x, int M, const uint16_t* bias, int activation,
+                          const uint16_t* residual, void* stream);
+
+/* Layers of experts (no reference counterpart). A container holds the same linear layer of num_experts experts (1..512), their
+ * streams one after another behind `qweight`, each as in w4a16_weights_t. */
+typedef struct w4a16_experts {
+  uint32_t* qweight;
+  int num_experts, out_f, in_f, group_size, num_groups;
+} w4a16_experts_t;
+int w4a16_experts_alloc(w4a16_experts_t* w, int num_experts, int out_f, int in_f, int group_size, void* stream);
+int w4a16_experts_free(w4a16_experts_t* w);
+/* One expert of the container as a layer of its own: for w4a16_repack_into(_swiglu), w4a16_dequant_rows and every matmul call.
+ * The view owns nothing (w4a16_weights_free refuses it) and ends with the container. */
+int w4a16_experts_view(const w4a16_experts_t* w, int expert, w4a16_weights_t* view);
+/* Products grouped by expert, ragged sizes: slot p of expert e, offsets[e] <= p < offsets[e + 1], is
+ *   y[p] = act(W_e x[x_rows[p]] + bias_e)      (x_rows NULL: x[p])
+ *   y       bf16 [slots][out_f] (SWIGLU: [slots][out_f / 2]); rows behind offsets[num_experts] stay as they were
+ *   x       bf16 [x_tokens][in_f]; x_rows int32 [slots], each in [0, x_tokens)
+ *   offsets int32 [num_experts + 1], ascending from 0, the last at most `slots`, as w4a16_route writes them. Both tables are read on the
+ *           device; bounds and rows outside these ranges are clamped into them, so that no call leaves its buffers, but what
+ *           it then writes into y is not specified.
+ *   bias    bf16 [num_experts][out_f] or NULL; activation, precision and alignment as in w4a16_linear_epilogue.
+ * Experts without slots cost nothing. One launch. y must not overlap x or bias. */
+int w4a16_experts_linear(uint16_t* y, const w4a16_experts_t* w, const uint16_t* x, int x_tokens, const int32_t* x_rows,
+                         const int32_t* offsets, int slots, const uint16_t* bias, int activation, void* stream);
+/* Router: of each token's num_experts logits (fp32 or bf16, [T][num_experts]) the top_k largest (1..16), ties to the lowest index.
+ * A logit of -inf or NaN is never picked, so a row may have fewer picks, or none (padding): the rest of its picks are empty.
+ *   ids     int32 [T][top_k]  experts in descending order of their logits; empty: -1
+ *   weights fp32  [T][top_k]  exp(logit) over the sum of exp, over the picks if `renormalize`, else over all experts; empty: 0
+ *   slots   int32 [T][top_k]  the picks sorted by expert, within an expert by token; empty: -1
+ *   offsets int32 [num_experts + 1]  first slot of every expert, then the number of slots
+ *   rows    int32 [T * top_k] the token of every slot; entries behind the last slot stay as they were
+ * (a logit of +inf counts as the largest finite one). Results are the same in every run. `workspace`: at least
+ * w4a16_route_workspace(T, num_experts) bytes, 4-byte aligned, one call in flight per workspace. T = 0 writes the offsets. */
+size_t w4a16_route_workspace(int max_tokens, int num_experts);
+int w4a16_route(int32_t* ids, float* weights, int32_t* offsets, int32_t* slots, int32_t* rows, const void* logits, int logits_are_f32,
+                int T, int num_experts, int top_k, int renormalize, void* workspace, size_t workspace_bytes, void* stream);
+/* The experts' outputs back to their tokens: y[t] = residual[t] + sum over j of weights[t][j] * parts[slots[t][j]], summed in fp32 in
+ * the order of j and rounded once. Picks whose slot is not in [0, parts_rows) count as empty. parts bf16 [parts_rows][hidden],
+ * y and residual (may be NULL, may be y itself) bf16 [T][hidden], all 16-byte aligned; hidden a multiple of 8, top_k 1..16. */
+int w4a16_experts_combine(uint16_t* y, const uint16_t* parts, int parts_rows, const int32_t* slots, const float* weights,
+                          const uint16_t* residual, int T, int top_k, int hidden, void* stream);
+
 /* w4a16_dequant_rows (gemm_w4a16.cuh:45-48, gemm_w4a16.cu:15-38,56-61): rows
  * [row0,row0+nrows) -> row-major bf16 [nrows][in_f], bf16(float(q-zp)*float(s)). */
 int w4a16_dequant_rows(uint16_t* dst, const w4a16_weights_t* w, int row0, int nrows, void* stream);

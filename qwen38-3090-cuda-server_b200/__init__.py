@@ -52,6 +52,12 @@ class W8Weights(C.Structure):
         return self.out_f * self.in_f + self.out_f * self.num_groups * 2
 
 
+class Experts(C.Structure):
+    """w4a16_experts_t: one linear layer of every expert."""
+    _fields_ = [("qweight", C.c_void_p), ("num_experts", C.c_int), ("out_f", C.c_int), ("in_f", C.c_int),
+                ("group_size", C.c_int), ("num_groups", C.c_int)]
+
+
 class Comm(C.Structure):
     """w4a16_comm_t: every rank's 256-byte flag block (peer-mapped), number of ranks, this rank."""
     _fields_ = [("blocks", C.c_void_p * 8), ("nranks", C.c_int), ("rank", C.c_int)]
@@ -124,6 +130,17 @@ _SIGNATURES = {
                                      C.c_void_p, C.c_int, C.POINTER(Scratch), C.c_void_p]),
     "w4a16_repack_into_swiglu": (C.c_int, [C.POINTER(Weights), C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int,
                                            C.c_int, C.c_void_p]),
+    "w4a16_linear_epilogue": (C.c_int, [C.c_void_p, C.POINTER(Weights), C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_void_p,
+                                        C.c_void_p]),
+    "w4a16_experts_alloc": (C.c_int, [C.POINTER(Experts), C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p]),
+    "w4a16_experts_free": (C.c_int, [C.POINTER(Experts)]),
+    "w4a16_experts_view": (C.c_int, [C.POINTER(Experts), C.c_int, C.POINTER(Weights)]),
+    "w4a16_experts_linear": (C.c_int, [C.c_void_p, C.POINTER(Experts), C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int,
+                                       C.c_void_p, C.c_int, C.c_void_p]),
+    "w4a16_route_workspace": (C.c_size_t, [C.c_int, C.c_int]),
+    "w4a16_route": (C.c_int, [C.c_void_p] * 6 + [C.c_int] * 5 + [C.c_void_p, C.c_size_t, C.c_void_p]),
+    "w4a16_experts_combine": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int,
+                                        C.c_int, C.c_void_p]),
     "w4a16_shard_rows": (C.c_int, [C.c_int, C.c_int, C.c_int, C.POINTER(C.c_int), C.POINTER(C.c_int)]),
     "w4a16_gemm_skinny_sharded": (C.c_int, [C.POINTER(C.c_void_p), C.c_int, C.c_int, C.c_int, C.c_int,
                                             C.POINTER(Weights), C.c_void_p, C.c_int, C.POINTER(Scratch),
@@ -366,6 +383,117 @@ def linear_fused(y, w: Weights, x, M: int, s: Scratch, ln_weight=None, ln_eps: f
     """A linear layer with RMSNorm in front and / or SwiGLU or the residual add behind, in one call."""
     check(lib().w4a16_linear_fused(_ptr(y), C.byref(w), _ptr(x), M, _ptr(ln_weight), ln_eps, _ptr(xn_out), epilogue,
                                    C.byref(s), _stream(stream)))
+
+
+# --------------------------------------------------------------------- layers with an epilogue, layers of experts
+ACT_NONE, ACT_SILU, ACT_GELU, ACT_GELU_TANH, ACT_SWIGLU = 0, 1, 2, 3, 4
+
+
+def _check_tensor(what: str, t, dtypes, rows: int, cols=None):
+    """`t` (None passes) must be contiguous, on the current device, of one of `dtypes` (names) and hold rows [x cols] elements."""
+    if t is None:
+        return
+    if str(t.dtype)[6:] not in dtypes:
+        raise W4A16Error(-1, f"{what}: {t.dtype}, not {' or '.join(dtypes)}")
+    if t.numel() != (rows if cols is None else rows * cols) or not t.is_contiguous():
+        raise W4A16Error(-1, f"{what}: {tuple(t.shape)}, not contiguous {rows if cols is None else (rows, cols)}")
+    if t.get_device() != _device():
+        raise W4A16Error(-1, f"{what}: on {t.device}, the current device is {_device()}")
+
+
+def _device() -> int:
+    if _torch is None:
+        _stream()
+    return _torch.cuda.current_device()
+
+
+def linear_epilogue(y, w: Weights, x, M: int, bias=None, activation: int = ACT_NONE, residual=None, stream=None):
+    """y = act(x W^T + bias) + residual for any M; ACT_SWIGLU: w repacked by awq_repack_into_swiglu, y [M, out_f / 2], bias
+    [gate | up]. residual may be y."""
+    cols = w.out_f // 2 if activation == ACT_SWIGLU else w.out_f
+    _check_tensor("linear_epilogue: x", x, ("bfloat16",), M, w.in_f)
+    _check_tensor("linear_epilogue: y", y, ("bfloat16",), M, cols)
+    _check_tensor("linear_epilogue: bias", bias, ("bfloat16",), w.out_f)
+    _check_tensor("linear_epilogue: residual", residual, ("bfloat16",), M, cols)
+    check(lib().w4a16_linear_epilogue(_ptr(y), C.byref(w), _ptr(x), M, _ptr(bias), activation, _ptr(residual), _stream(stream)))
+
+
+def experts_alloc(num_experts: int, out_f: int, in_f: int, group_size: int = 128) -> Experts:
+    w = Experts()
+    check(lib().w4a16_experts_alloc(C.byref(w), num_experts, out_f, in_f, group_size, _stream()))
+    return w
+
+
+def experts_free(w: Experts):
+    check(lib().w4a16_experts_free(C.byref(w)))
+
+
+def experts_view(w: Experts, expert: int) -> Weights:
+    """One expert as a layer of its own, for awq_repack_into(_swiglu) and every other call; it owns nothing."""
+    view = Weights()
+    check(lib().w4a16_experts_view(C.byref(w), expert, C.byref(view)))
+    return view
+
+
+def experts_linear(y, w: Experts, x, offsets, x_rows=None, bias=None, activation: int = ACT_NONE, stream=None):
+    """y[p] = act(W_e x[x_rows[p]] + bias[e]) for the slots offsets[e] <= p < offsets[e + 1] of every expert e (x_rows None: x[p]).
+    y [slots, out_f] (ACT_SWIGLU: out_f / 2 columns), x [tokens, in_f], offsets int32 [experts + 1], x_rows int32 [slots], as
+    `route` gives them; rows of y behind the last slot stay as they were."""
+    slots = y.shape[0]
+    _check_tensor("experts_linear: y", y, ("bfloat16",), slots, w.out_f // 2 if activation == ACT_SWIGLU else w.out_f)
+    _check_tensor("experts_linear: x", x, ("bfloat16",), x.shape[0], w.in_f)
+    _check_tensor("experts_linear: offsets", offsets, ("int32",), w.num_experts + 1)
+    _check_tensor("experts_linear: x_rows", x_rows, ("int32",), slots)
+    _check_tensor("experts_linear: bias", bias, ("bfloat16",), w.num_experts, w.out_f)
+    check(lib().w4a16_experts_linear(_ptr(y), C.byref(w), _ptr(x), x.shape[0], _ptr(x_rows), _ptr(offsets), slots, _ptr(bias),
+                                     activation, _stream(stream)))
+
+
+class Route:
+    """What `route` writes, for up to max_tokens tokens: ids, weights, slots [max_tokens, top_k], offsets [experts + 1],
+    rows [max_tokens * top_k], and its workspace. One call in flight per Route."""
+
+    def __init__(self, max_tokens: int, num_experts: int, top_k: int):
+        import torch
+        self.max_tokens, self.num_experts, self.top_k = max_tokens, num_experts, top_k
+
+        def make(*shape, dtype=torch.int32):
+            return torch.zeros(shape, dtype=dtype, device="cuda")
+
+        self.ids, self.slots, self.weights = make(max_tokens, top_k), make(max_tokens, top_k), make(max_tokens, top_k, dtype=torch.float32)
+        self.offsets, self.rows = make(num_experts + 1), make(max_tokens * top_k)
+        self.workspace_bytes = lib().w4a16_route_workspace(max_tokens, num_experts)
+        self.workspace = make(self.workspace_bytes // 4)
+
+
+def route_alloc(max_tokens: int, num_experts: int, top_k: int) -> Route:
+    return Route(max_tokens, num_experts, top_k)
+
+
+def route(r: Route, logits, renormalize: bool = True, stream=None):
+    """Router logits [T, experts] (fp32 or bf16) -> the first T rows of r.ids, r.weights and r.slots, r.offsets and the first
+    r.offsets[-1] entries of r.rows. Logits of -inf or NaN are never picked; empty picks have id -1, weight 0, slot -1."""
+    T = logits.shape[0]
+    if T > r.max_tokens:
+        raise W4A16Error(-1, f"route: {T} tokens, room for {r.max_tokens}")
+    _check_tensor("route: logits", logits, ("float32", "bfloat16"), T, r.num_experts)
+    _check_tensor("route: workspace", r.workspace, ("int32",), r.workspace_bytes // 4)
+    check(lib().w4a16_route(_ptr(r.ids), _ptr(r.weights), _ptr(r.offsets), _ptr(r.slots), _ptr(r.rows), _ptr(logits),
+                            1 if logits.element_size() == 4 else 0, T, r.num_experts, r.top_k, 1 if renormalize else 0,
+                            _ptr(r.workspace), r.workspace_bytes, _stream(stream)))
+
+
+def experts_combine(y, parts, slots, weights, residual=None, stream=None):
+    """y[t] = residual[t] + sum over j of weights[t, j] * parts[slots[t, j]] (slots outside parts are empty). y, residual [T, hidden],
+    parts [any, hidden], slots int32 and weights fp32 [T, top_k]; residual may be y."""
+    (T, hidden), top_k = y.shape, slots.shape[1]
+    _check_tensor("experts_combine: y", y, ("bfloat16",), T, hidden)
+    _check_tensor("experts_combine: parts", parts, ("bfloat16",), parts.shape[0], hidden)
+    _check_tensor("experts_combine: slots", slots, ("int32",), T, top_k)
+    _check_tensor("experts_combine: weights", weights, ("float32",), T, top_k)
+    _check_tensor("experts_combine: residual", residual, ("bfloat16",), T, hidden)
+    check(lib().w4a16_experts_combine(_ptr(y), _ptr(parts), parts.shape[0], _ptr(slots), _ptr(weights), _ptr(residual), T, top_k,
+                                      hidden, _stream(stream)))
 
 
 def device_status() -> int:

@@ -33,6 +33,7 @@ struct DeviceInfo {
   int device = -1;
   int sms = 0;
   int smem_optin = 0;
+  int smem_per_sm = 0, smem_reserved = 0;  // shared memory of an SM, and what every CTA takes of it for itself
   int* status = nullptr;  // device address of the sticky status word (0 ok / W4A16_ETIMEOUT)
 };
 // Cached per device; returns nullptr (and sets the error) on failure.
@@ -342,6 +343,34 @@ __device__ __forceinline__ unsigned signal_whole_launch(unsigned* local, unsigne
   fence_sys();
   for (int r = 0; r < n; ++r) red_add_relaxed_sys(peers[r] + rank, kCommUnit);
   return seq;
+}
+
+// ---- thread-block clusters ----
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t map_to_rank(uint32_t saddr, uint32_t rank) {
+  uint32_t d;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(d) : "r"(saddr), "r"(rank));
+  return d;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float2 ld_cluster_f32x2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
 }
 
 __device__ __forceinline__ float bf16_bits_to_float(uint16_t h) {

@@ -1,0 +1,464 @@
+// Linear layers over ragged sets of few tokens, for sm_100a: y[p] = bf16(act(x[row of p] W_e^T + bias_e) + residual[p]).
+// The dense layer with an epilogue (one set) and the products grouped by expert; int4 weights, groups of 128.
+//
+// Mathematics: W = bf16((q - z) s), the value w4a16_dequant_rows gives, made in registers with packed bf16 arithmetic (every
+// step but the last exact) and multiplied by the bf16 activations on the tensor cores with fp32 sums, whatever the number of tokens.
+//
+// A unit of work is a 128-row tile of a set's weights with up to NT of its tokens (NT = 8, 16 or 32). A CTA takes a unit; where there are
+// few units, a cluster of S CTAs shares one, each a range of k groups, and adds up through distributed shared memory in a
+// fixed order (bitwise reproducible). In a CTA
+//   * one producer warp fills a ring of stages, a k group each: the 8576-byte weight block by one bulk copy (cp.async.bulk), each
+//     token's 128 activations by another, so that rows are gathered in the load;
+//   * eight consumer warps take 32 rows x 64 k each: mma.sync m16n8k16 with the weights as the A operand straight from the
+//     expansion. The fragments' k order is free as long as both operands share it, so a lane takes 16 consecutive k of
+//     its row (8 bytes of codes) and of its token (two 16-byte loads).
+#include <atomic>
+#include <climits>
+#include <cstring>
+
+#include "ragged.cuh"
+
+namespace w4a16 {
+namespace {
+
+constexpr int kRCons = 8;                        // consumer warps
+constexpr int kRThreads = (kRCons + 1) * 32;
+constexpr int kRMaxDepth = 16;                   // ring stages at most
+constexpr int kXPitch = 272;                     // bytes of a token's 128 activations in a stage: 16 more than they are, against bank conflicts
+constexpr uint32_t kRSpin = 1u << 20;
+
+struct RaggedParams {
+  RaggedCall c;
+  int row_tiles, splits, depth;
+  int* status;
+};
+
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Where unit u of the launch lies: set, first slot, tokens, row tile. The chunks of one row tile are neighbours, so that its
+// weights come from HBM once. `e` moves on only (a CTA's units ascend).
+struct Unit {
+  int e, slot0, n, rt;
+};
+template <int NT>
+__device__ __forceinline__ Unit unit_of(int u, int& e, const int* first, const int2* bounds, int sets) {
+  while (e + 1 < sets && u >= first[e + 1]) ++e;
+  const int n = bounds[e].y - bounds[e].x, chunks = (n + NT - 1) / NT, at = u - first[e];
+  Unit t;
+  t.e = e;
+  t.rt = at / chunks;
+  const int c = at - t.rt * chunks;
+  t.slot0 = bounds[e].x + c * NT;
+  t.n = min(NT, n - c * NT);
+  return t;
+}
+
+template <int NT>
+__host__ __device__ constexpr int stage_bytes() {
+  return kTileGroupBytes + NT * kXPitch;
+}
+template <int NT>
+__host__ __device__ constexpr int sum_bytes() {  // the two k halves' sums: [2][NT tokens][128 rows] floats
+  return 2 * NT * kTileRows * 4;
+}
+
+template <int NT>
+__global__ void __launch_bounds__(kRThreads, 2) k_ragged(const __grid_constant__ RaggedParams p) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  const RaggedCall& c = p.c;
+  float* sums = reinterpret_cast<float*>(smem);
+  uint8_t* ring = smem + sum_bytes<NT>();
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + p.depth * stage_bytes<NT>());
+  int2* bounds = reinterpret_cast<int2*>(bars + 2 * kRMaxDepth);
+  int* first = reinterpret_cast<int*>(bounds + c.sets);  // [sets + 1] units in front of each set
+
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  const int S = p.splits, split = S > 1 ? static_cast<int>(cluster_rank()) : 0;
+  const int cluster = blockIdx.x / S, nclusters = gridDim.x / S;
+  const uint32_t ring_a = smem_u32(ring), full_a = smem_u32(bars), empty_a = full_a + kRMaxDepth * 8;
+  if (tid == 0) {
+    for (int i = 0; i < p.depth; ++i) {
+      mbar_init(full_a + i * 8, 1);
+      mbar_init(empty_a + i * 8, kRCons);
+    }
+    fence_mbar_init();
+  }
+  pdl_launch_dependents();
+  pdl_wait();  // offsets, rows and activations come from the kernels in front
+  if (warp == 0) {
+    // units of every set: ceil(tokens / NT) chunks of each row tile
+    int run = 0;
+    for (int e0 = 0; e0 < c.sets; e0 += 32) {
+      const int e = e0 + lane;
+      int2 b = make_int2(0, 0);
+      if (e < c.sets) {
+        b = c.offsets ? set_slots(c.offsets, e, c.slots) : make_int2(0, c.slots);
+        bounds[e] = b;
+      }
+      const int mine = (b.y - b.x + NT - 1) / NT * p.row_tiles;
+      int upto = mine;
+#pragma unroll
+      for (int d = 1; d < 32; d *= 2) {
+        const int v = __shfl_up_sync(0xffffffffu, upto, d);
+        if (lane >= d) upto += v;
+      }
+      if (e < c.sets) first[e] = run + upto - mine;
+      run += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    if (lane == 0) first[c.sets] = run;
+  }
+  __syncthreads();
+  const int units = first[c.sets];
+  const int g0 = c.G * split / S, g1 = c.G * (split + 1) / S;
+  bool dead = false;
+  int e = 0, st = 0;
+
+  if (warp == kRCons) {
+    // ================================================================ producer
+    uint32_t ph = 1;
+    int issued = 0;
+    for (int u = cluster; !dead && u < units; u += nclusters) {
+      const Unit t = unit_of<NT>(u, e, first, bounds, c.sets);
+      const uint8_t* src = c.stream + static_cast<size_t>(t.e) * c.set_bytes + (static_cast<size_t>(t.rt) * c.G + g0) * kTileGroupBytes;
+      int row = t.slot0 + min(lane, t.n - 1);
+      if (c.x_rows) row = __ldcg(c.x_rows + row);
+      row = min(max(row, 0), c.x_tokens - 1);  // (no read outside x, whatever the rows hold)
+      const uint16_t* xr = c.x + static_cast<size_t>(row) * c.K + static_cast<size_t>(g0) * kGroup;
+      for (int g = g0; g < g1; ++g, src += kTileGroupBytes, xr += kGroup) {
+        if (!warp_agrees(mbar_wait_bounded_relaxed(empty_a + st * 8, ph, kRSpin))) {
+          dead = true;
+          break;
+        }
+        const uint32_t dst = ring_a + st * stage_bytes<NT>();
+        if (lane == 0) {
+          mbar_expect_tx(full_a + st * 8, kTileGroupBytes + t.n * kGroup * 2);
+          bulk_g2s(dst, src, kTileGroupBytes, full_a + st * 8);
+        }
+        __syncwarp();
+        if (lane < t.n) bulk_g2s(dst + kTileGroupBytes + lane * kXPitch, xr, kGroup * 2, full_a + st * 8);
+        ++issued;
+        if (++st == p.depth) {
+          st = 0;
+          ph ^= 1;
+        }
+      }
+    }
+    if (dead) {  // the copies in flight still have to land
+      if (lane == 0) atomicExch(p.status, W4A16_ETIMEOUT);
+      for (int i = 0; i < p.depth && i < issued; ++i) mbar_wait_bounded_relaxed(full_a + i * 8, i < st ? ph ^ 1u : ph, 1u << 10);
+    }
+    __syncwarp();
+    if (S > 1) {
+      cluster_sync();
+      cluster_sync();
+    }
+    return;
+  }
+
+  // ================================================================ consumers
+  const int half = warp & 1, r0 = (warp >> 1) * 32 + (lane >> 2), t4 = lane & 3;
+  const int chunk = 2 * half + (t4 >> 1);
+  const uint32_t w_off = chunk * kChunkBytes + (t4 & 1) * 8;
+  const uint32_t x_off = kTileGroupBytes + (lane >> 2) * kXPitch + (half * 64 + t4 * 16) * 2;
+  uint32_t ph = 0;
+  for (int u = cluster; u < units; u += nclusters) {
+    const Unit t = unit_of<NT>(u, e, first, bounds, c.sets);
+    float acc[2][NT / 8][4] = {};
+    for (int g = g0; g < g1 && !dead; ++g) {
+      if (!warp_agrees(mbar_wait_bounded(full_a + st * 8, ph, kRSpin))) {
+        dead = true;
+        break;
+      }
+      const uint8_t* blk = ring + st * stage_bytes<NT>();
+      uint2 w[4];
+      uint32_t zpair[4], spair[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = r0 + 8 * i;
+        w[i] = *reinterpret_cast<const uint2*>(blk + w_off + weight_slot(r, chunk) * 16);
+        const uint32_t sc = reinterpret_cast<const uint16_t*>(blk + kTgScaleOff)[r];
+        spair[i] = sc | (sc << 16);
+        zpair[i] = __byte_perm(blk[kTgZpOff + r], 0x43434343u, 0x4040);  // bf16 pair (128 + zp, 128 + zp)
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {  // 8 of the lane's 16 k: one word of codes, one 16-byte load per token
+        uint32_t a[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t word = h ? w[i].y : w[i].x;
+#pragma unroll
+          for (int pp = 0; pp < 4; ++pp)  // (128 + q) - (128 + zp) is exact, the product rounds once
+            a[i][pp] = mul_bf16x2(sub_bf16x2(((word >> (4 * pp)) & 0x000F000Fu) | 0x43004300u, zpair[i]), spair[i]);
+        }
+#pragma unroll
+        for (int j = 0; j < NT / 8; ++j) {
+          if (j == 0 || 8 * j < t.n) {
+            const uint4 b = *reinterpret_cast<const uint4*>(blk + x_off + 8 * j * kXPitch + 16 * h);
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+              mma_bf16(acc[m][j], a[2 * m][0], a[2 * m + 1][0], a[2 * m][1], a[2 * m + 1][1], b.x, b.y);
+              mma_bf16(acc[m][j], a[2 * m][2], a[2 * m + 1][2], a[2 * m][3], a[2 * m + 1][3], b.z, b.w);
+            }
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(empty_a + st * 8);
+      if (++st == p.depth) {
+        st = 0;
+        ph ^= 1;
+      }
+    }
+    // ---- the halves' (and the splits') sums meet in shared memory; every output is added up in one order and finished by one thread
+    named_bar_sync(1, kRCons * 32);  // the unit before has been read out
+#pragma unroll
+    for (int j = 0; j < NT / 8; ++j)
+      if (j == 0 || 8 * j < t.n)
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            sums[(half * NT + 8 * j + 2 * t4 + (i & 1)) * kTileRows + r0 + 16 * m + 8 * (i >> 1)] = acc[m][j][i];
+    if (S > 1) cluster_sync();
+    named_bar_sync(1, kRCons * 32);
+    const int pairs = t.n * (kTileRows / 2);
+    for (int i = tid + split * kRCons * 32; i < pairs && !dead; i += S * kRCons * 32) {
+      const int tok = i / (kTileRows / 2), r = 2 * (i % (kTileRows / 2)), row = t.rt * kTileRows + r;
+      if (row >= c.N) continue;
+      float v0 = 0.f, v1 = 0.f;
+      for (int s = 0; s < S; ++s) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float* at = sums + (h * NT + tok) * kTileRows + r;
+          const float2 v = S > 1 ? ld_cluster_f32x2(map_to_rank(smem_u32(at), s)) : *reinterpret_cast<const float2*>(at);
+          v0 += v.x;
+          v1 += v.y;
+        }
+      }
+      if (c.bias) {
+        const uint16_t* b = c.bias + static_cast<size_t>(t.e) * c.N;
+        v0 += bf16_bits_to_float(b[bias_index(row, c.N, c.act)]);
+        v1 += bf16_bits_to_float(b[bias_index(row + 1, c.N, c.act)]);
+      }
+      const size_t line = static_cast<size_t>(t.slot0 + tok) * c.ny;
+      if (c.act == W4A16_ACT_SWIGLU) {
+        const size_t o = line + (row >> 1);
+        float v = logistic_times(v0, v0) * v1;
+        if (c.residual) v += bf16_bits_to_float(c.residual[o]);
+        c.y[o] = float_to_bf16_bits(v);
+      } else {
+        const size_t o = line + row;
+        v0 = activate(v0, c.act);
+        v1 = activate(v1, c.act);
+        if (c.residual) {
+          const uint32_t r2 = *reinterpret_cast<const uint32_t*>(c.residual + o);
+          v0 += bf16_bits_to_float(static_cast<uint16_t>(r2));
+          v1 += bf16_bits_to_float(static_cast<uint16_t>(r2 >> 16));
+        }
+        *reinterpret_cast<uint32_t*>(c.y + o) = float_to_bf16_bits(v0) | (static_cast<uint32_t>(float_to_bf16_bits(v1)) << 16);
+      }
+    }
+    if (S > 1) break;  // (a cluster takes one unit)
+  }
+  if (dead && lane == 0) atomicExch(p.status, W4A16_ETIMEOUT);
+  __syncwarp();
+  if (S > 1) {
+    if (cluster >= units) cluster_sync();
+    cluster_sync();  // nobody leaves while its sums may still be read
+  }
+}
+
+template <int NT>
+int launch_ragged(RaggedParams& p, const DeviceInfo* di, int max_units, bool weights_first, cudaStream_t st) {
+  const int fixed = sum_bytes<NT>() + 2 * kRMaxDepth * 8 + p.c.sets * 8 + (p.c.sets + 1) * 4;
+  const int room = (di->smem_per_sm / 2 - di->smem_reserved - fixed) / stage_bytes<NT>();
+  p.depth = room < kRMaxDepth ? room : kRMaxDepth;
+  const int smem = fixed + p.depth * stage_bytes<NT>();
+  static std::atomic<bool> ready[64];
+  if (!ready[di->device & 63].load(std::memory_order_acquire)) {
+    W4_CUDA(cudaFuncSetAttribute(k_ragged<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, di->smem_optin));
+    ready[di->device & 63].store(true, std::memory_order_release);
+  }
+  const int slots = 2 * di->sms;
+  int S = slots / max_units;
+  S = S > 8 ? 8 : S;
+  S = S > p.c.G / 2 ? p.c.G / 2 : S;
+  p.splits = S < 1 ? 1 : S;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[2];
+  cfg.gridDim = dim3(p.splits > 1 ? p.splits * max_units : (max_units < slots ? max_units : slots));
+  cfg.blockDim = dim3(kRThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = at;
+  cfg.numAttrs = 0;
+  if (p.splits > 1) {
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = p.splits;
+    at[0].val.clusterDim.y = 1;
+    at[0].val.clusterDim.z = 1;
+    cfg.numAttrs = 1;
+  }
+  if (pdl_enabled()) {
+    at[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++cfg.numAttrs;
+  }
+  (void)weights_first;
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, k_ragged<NT>, p);
+  return err == cudaSuccess ? W4A16_OK : fail(W4A16_ECUDA, "linear: launch: %s", cudaGetErrorString(err));
+}
+
+bool aligned16(const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; }
+
+// Checks what both entry points share and enqueues the call.
+int run_ragged(RaggedCall& c, const char* who, cudaStream_t st) {
+  W4_REQUIRE(c.act >= W4A16_ACT_NONE && c.act <= W4A16_ACT_SWIGLU, "%s: unknown activation %d", who, c.act);
+  W4_REQUIRE(c.act != W4A16_ACT_SWIGLU || c.N % 32 == 0, "%s: out_f %d must be a multiple of 32 (gate, up interleaved)", who, c.N);
+  if (c.slots == 0) return W4A16_OK;
+  W4_REQUIRE(c.x != nullptr && c.y != nullptr && c.x_tokens > 0, "%s: null or empty matrix", who);
+  W4_REQUIRE(aligned16(c.x) && aligned16(c.y) && aligned16(c.residual), "%s: x, y and residual must be 16-byte aligned", who);
+  W4_REQUIRE((reinterpret_cast<uintptr_t>(c.bias) & 1) == 0, "%s: bias not 2-byte aligned", who);
+  W4_REQUIRE(((reinterpret_cast<uintptr_t>(c.offsets) | reinterpret_cast<uintptr_t>(c.x_rows)) & 3) == 0,
+             "%s: offsets or x_rows not 4-byte aligned", who);
+  c.ny = c.act == W4A16_ACT_SWIGLU ? c.N / 2 : c.N;
+  const size_t xb = static_cast<size_t>(c.x_tokens) * c.K * 2, yb = static_cast<size_t>(c.slots) * c.ny * 2;
+  W4_REQUIRE(ranges_apart(c.x, xb, c.y, yb), "%s: y overlaps x", who);
+  W4_REQUIRE(c.residual == nullptr || c.residual == c.y || ranges_apart(c.residual, yb, c.y, yb), "%s: residual overlaps y but is not y", who);
+  W4_REQUIRE(c.bias == nullptr || ranges_apart(c.bias, static_cast<size_t>(c.sets) * c.N * 2, c.y, yb), "%s: y overlaps bias", who);
+  const DeviceInfo* di = device_info();
+  if (!di) return W4A16_ECUDA;
+  RaggedParams p = {};
+  p.c = c;
+  p.row_tiles = (c.N + kTileRows - 1) / kTileRows;
+  p.status = di->status;
+  // chunks of NT tokens at most: every set with tokens has one more than its whole ones
+  const int used = c.slots < c.sets ? c.slots : c.sets;
+  const int mean = (c.slots + c.sets - 1) / c.sets;
+  const int nt = mean <= 4 || (c.sets == 1 && c.slots <= 8) ? 8 : mean <= 10 || (c.sets == 1 && c.slots <= 16) ? 16 : 32;
+  const long long chunks = c.sets == 1 ? (c.slots + nt - 1) / nt : used + (c.slots - used) / nt;
+  const long long units = chunks * p.row_tiles;
+  W4_REQUIRE(units <= INT_MAX, "%s: %d slots x %d rows are too many for one call", who, c.slots, c.N);
+  const int max_units = static_cast<int>(units);
+  const bool dense = c.offsets == nullptr;
+  if (nt == 8) return launch_ragged<8>(p, di, max_units, dense, st);
+  if (nt == 16) return launch_ragged<16>(p, di, max_units, dense, st);
+  return launch_ragged<32>(p, di, max_units, dense, st);
+}
+
+int check_experts(const w4a16_experts_t* w) {
+  W4_REQUIRE(w != nullptr && w->qweight != nullptr && aligned16(w->qweight), "experts: null or misaligned weights");
+  W4_REQUIRE(w->group_size == kGroup && w->in_f > 0 && w->in_f % kGroup == 0 && w->num_groups == w->in_f / kGroup,
+             "experts: in_f %d, group_size %d, %d groups", w->in_f, w->group_size, w->num_groups);
+  W4_REQUIRE(w->out_f > 0 && w->out_f % kRowGranule == 0, "experts: out_f %d not a positive multiple of 16", w->out_f);
+  W4_REQUIRE(w->num_experts >= 1 && w->num_experts <= kMaxSets, "experts: %d experts (1..%d)", w->num_experts, kMaxSets);
+  return W4A16_OK;
+}
+
+}  // namespace
+}  // namespace w4a16
+
+using namespace w4a16;
+
+extern "C" {
+
+int w4a16_linear_epilogue(uint16_t* y, const w4a16_weights_t* w, const uint16_t* x, int M, const uint16_t* bias, int activation,
+                          const uint16_t* residual, void* stream) {
+  if (int rc = check_weights(w)) return rc;
+  W4_REQUIRE(M >= 0, "linear_epilogue: M = %d", M);
+  RaggedCall c = {};
+  c.stream = reinterpret_cast<const uint8_t*>(w->qweight);
+  c.sets = 1;
+  c.N = w->out_f;
+  c.K = w->in_f;
+  c.G = w->num_groups;
+  c.x = x;
+  c.x_tokens = M;
+  c.slots = M;
+  c.bias = bias;
+  c.act = activation;
+  c.residual = residual;
+  c.y = y;
+  return run_ragged(c, "linear_epilogue", static_cast<cudaStream_t>(stream));
+}
+
+int w4a16_experts_alloc(w4a16_experts_t* w, int num_experts, int out_f, int in_f, int group_size, void* stream) {
+  W4_REQUIRE(w != nullptr, "experts_alloc: null struct");
+  w4a16_experts_t d = {};
+  d.qweight = reinterpret_cast<uint32_t*>(16);  // (for the check; replaced below)
+  d.num_experts = num_experts;
+  d.out_f = out_f;
+  d.in_f = in_f;
+  d.group_size = group_size;
+  d.num_groups = group_size > 0 ? in_f / group_size : 0;
+  memset(w, 0, sizeof *w);
+  if (int rc = check_experts(&d)) return rc;
+  const size_t bytes = stream_bytes(out_f, d.num_groups) * num_experts;
+  void* q = nullptr;
+  cudaError_t e = cudaMalloc(&q, bytes);
+  if (e == cudaSuccess && out_f % kTileRows != 0) {
+    // rows past out_f in every expert's last tile: zero scales (see w4a16_weights_alloc)
+    e = cudaMemsetAsync(q, 0, bytes, static_cast<cudaStream_t>(stream));
+    note_weight_write(static_cast<cudaStream_t>(stream));
+  }
+  if (e != cudaSuccess) {
+    cudaFree(q);
+    return fail(W4A16_ECUDA, "experts_alloc(%d x %d x %d): %s", num_experts, out_f, in_f, cudaGetErrorString(e));
+  }
+  d.qweight = static_cast<uint32_t*>(q);
+  *w = d;
+  return W4A16_OK;
+}
+
+int w4a16_experts_view(const w4a16_experts_t* w, int expert, w4a16_weights_t* view) {
+  if (int rc = check_experts(w)) return rc;
+  W4_REQUIRE(view != nullptr, "experts_view: null struct");
+  W4_REQUIRE(expert >= 0 && expert < w->num_experts, "experts_view: expert %d of %d", expert, w->num_experts);
+  uint8_t* q = reinterpret_cast<uint8_t*>(w->qweight) + stream_bytes(w->out_f, w->num_groups) * expert;
+  view->qweight = reinterpret_cast<uint32_t*>(q);
+  view->scale = reinterpret_cast<uint16_t*>(q);  // nothing is read through these two; w4a16_weights_free knows a view by them
+  view->zp = q;
+  view->out_f = w->out_f;
+  view->in_f = w->in_f;
+  view->group_size = w->group_size;
+  view->num_groups = w->num_groups;
+  return W4A16_OK;
+}
+
+int w4a16_experts_free(w4a16_experts_t* w) {
+  W4_REQUIRE(w != nullptr, "experts_free: null struct");
+  cudaFree(w->qweight);
+  memset(w, 0, sizeof *w);
+  return W4A16_OK;
+}
+
+int w4a16_experts_linear(uint16_t* y, const w4a16_experts_t* w, const uint16_t* x, int x_tokens, const int32_t* x_rows,
+                         const int32_t* offsets, int slots, const uint16_t* bias, int activation, void* stream) {
+  if (int rc = check_experts(w)) return rc;
+  W4_REQUIRE(slots >= 0 && x_tokens >= 0, "experts_linear: %d slots, %d tokens", slots, x_tokens);
+  W4_REQUIRE(offsets != nullptr, "experts_linear: null offsets");
+  W4_REQUIRE(x_rows != nullptr || slots <= x_tokens, "experts_linear: %d slots of %d rows, without x_rows", slots, x_tokens);
+  RaggedCall c = {};
+  c.stream = reinterpret_cast<const uint8_t*>(w->qweight);
+  c.set_bytes = stream_bytes(w->out_f, w->num_groups);
+  c.sets = w->num_experts;
+  c.N = w->out_f;
+  c.K = w->in_f;
+  c.G = w->num_groups;
+  c.x = x;
+  c.x_tokens = x_tokens;
+  c.x_rows = x_rows;
+  c.offsets = offsets;
+  c.slots = slots;
+  c.bias = bias;
+  c.act = activation;
+  c.y = y;
+  return run_ragged(c, "experts_linear", static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

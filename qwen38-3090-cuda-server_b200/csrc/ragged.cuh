@@ -1,0 +1,55 @@
+// Linear layers over ragged sets of tokens with their epilogue: what the decode-side kernel (ragged.cu) and the prefill kernel
+// (prefill.cu) share. A dense layer is one set with all tokens.
+#pragma once
+#include "common.cuh"
+
+namespace w4a16 {
+
+// y[p] = bf16(act(x[row of p] W_e^T + bias_e) + residual[p]) for the slots p in [offsets[e], offsets[e + 1]) of every set e.
+struct RaggedCall {
+  const uint8_t* stream;     // the sets' weight streams one after another
+  size_t set_bytes;          // from one set's stream to the next
+  int sets, N, K, G;
+  const uint16_t* x;         // [x_tokens][K]
+  int x_tokens;
+  const int32_t* x_rows;     // row of x of every slot (null: slot p takes row p)
+  const int32_t* offsets;    // [sets + 1] on the device (null: one set with all slots)
+  int slots;
+  const uint16_t* bias;      // [sets][N] in the checkpoint's row order, or null
+  int act;
+  const uint16_t* residual;  // laid out as y, or null; may be y itself
+  uint16_t* y;               // [slots][ny]
+  int ny;                    // N, or N / 2 with the gated activation
+};
+
+#ifdef __CUDACC__
+// v / (1 + exp(-v)); the gated and the tanh form come back to it: 0.5 v (1 + tanh u) = v / (1 + exp(-2 u)) holds its precision where
+// the tanh is near -1. Two special-function instructions a value.
+__device__ __forceinline__ float logistic_times(float v, float u) { return __fdividef(v, 1.f + __expf(-u)); }
+
+// An activation that acts on each output by itself, in fp32.
+__device__ __forceinline__ float activate(float v, int act) {
+  if (act == W4A16_ACT_SILU) return logistic_times(v, v);
+  if (act == W4A16_ACT_GELU_TANH) return logistic_times(v, 1.5957691216f * (v + 0.044715f * v * v * v));  // 2 sqrt(2 / pi)
+  if (act == W4A16_ACT_GELU) return 0.5f * v * erfcf(-0.70710678119f * v);  // (1 + erf would cancel for negative v)
+  return v;
+}
+// Index of a container row's bias: with the gated activation rows alternate gate, up, gate, up ...; the bias is [gate | up].
+__device__ __forceinline__ int bias_index(int row, int N, int act) {
+  return act == W4A16_ACT_SWIGLU ? (row >> 1) + (row & 1) * (N >> 1) : row;
+}
+// The set's slots, whatever the offsets hold: within [0, slots], the end not before the beginning.
+__device__ __forceinline__ int2 set_slots(const int32_t* offsets, int e, int slots) {
+  const int lo = min(max(__ldcg(offsets + e), 0), slots);
+  return make_int2(lo, min(max(__ldcg(offsets + e + 1), lo), slots));
+}
+#endif
+
+inline bool ranges_apart(const void* a, size_t an, const void* b, size_t bn) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x + an <= y || y + bn <= x;
+}
+
+constexpr int kMaxSets = 512;  // experts of a container: their bounds are kept in shared memory
+
+}  // namespace w4a16

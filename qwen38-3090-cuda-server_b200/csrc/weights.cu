@@ -59,9 +59,11 @@ const DeviceInfo* device_info() {
   if (g_dev_ready[dev].load(std::memory_order_acquire)) return &d;
   std::lock_guard<std::mutex> lk(g_dev_mu);
   if (d.device != dev) {
-    int sms = 0, smem = 0;
+    int sms = 0, smem = 0, per_sm = 0, reserved = 0;
     if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
-        cudaDeviceGetAttribute(&smem, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev) != cudaSuccess) {
+        cudaDeviceGetAttribute(&smem, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&per_sm, cudaDevAttrMaxSharedMemoryPerMultiprocessor, dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&reserved, cudaDevAttrReservedSharedMemoryPerBlock, dev) != cudaSuccess) {
       set_error("cudaDeviceGetAttribute failed");
       return nullptr;
     }
@@ -72,6 +74,8 @@ const DeviceInfo* device_info() {
     }
     d.sms = sms;
     d.smem_optin = smem;
+    d.smem_per_sm = per_sm;
+    d.smem_reserved = reserved;
     d.status = st;
     d.device = dev;
     g_dev_ready[dev].store(true, std::memory_order_release);
@@ -364,6 +368,7 @@ int w4a16_repack_into_swiglu(const w4a16_weights_t* w, int dst_row_offset, const
 
 int w4a16_weights_free(w4a16_weights_t* w) {
   W4_REQUIRE(w != nullptr, "weights_free: null struct");
+  W4_REQUIRE(w->qweight == nullptr || static_cast<void*>(w->scale) != w->qweight, "weights_free: a view of an expert owns nothing");
   cudaFree(w->qweight);
   cudaFree(w->scale);
   cudaFree(w->zp);
