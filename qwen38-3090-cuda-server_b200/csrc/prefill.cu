@@ -43,7 +43,7 @@
 #include <cstring>
 #include <mutex>
 
-#include "common.cuh"
+#include "ragged.cuh"
 
 namespace w4a16 {
 namespace {
@@ -66,6 +66,7 @@ constexpr int kPMaxA = 6;                   // A slots, at most
 constexpr int kPBars = 2 * kPMaxWD + kPDone + kPMaxA + kPSteps + 2;
 // Tensor memory: the accumulator's TN columns, the rest are slots of the A operand, 64 columns per k group.
 __host__ __device__ constexpr int a_slots(int tn) { return tn <= 128 ? 6 : 4; }
+constexpr int kPSetsTN = 224;               // with sets: their table needs the room that 256 tokens take
 static_assert(128 + 6 * 64 <= 512 && 256 + 4 * 64 <= 512 && kPMaxA <= kPDone && kPSteps <= kPDone, "ring depths");
 
 struct PrefillParams {
@@ -85,7 +86,13 @@ struct PrefillParams {
   unsigned* comm_local;
   unsigned* comm_peers[8];
   int comm_n, comm_rank;
+  // layers with an epilogue and layers of experts
+  RaggedCall call;
 };
+
+// What an instance of the kernel does: the plain GEMM, a dense layer with bias, activation and residual in its epilogue, or
+// the same per set of tokens with its own weights (experts), rows gathered in the load.
+constexpr int kPlain = 0, kDense = 1, kSets = 2;
 
 __device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t d;
@@ -130,15 +137,24 @@ __device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* m
       "l"(map), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
+// Four rows of 64 k, each of its own, into 512 consecutive bytes (with the swizzle of their place in a 1024-byte atom).
+__device__ __forceinline__ void tma_gather_pair(uint32_t dst, const CUtensorMap* map, int x, const int4& rows, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2 "
+      "[%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(rows.x), "r"(rows.y), "r"(rows.z), "r"(rows.w), "r"(bar)
+      : "memory");
+}
 // K-major operand descriptor for a 128-byte-swizzled tile ([row][128 B], 8-row groups 1024 B apart)
 __device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t saddr) {
   return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(1) << 16) |
          (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 
-// A tile: its row pair, first token and the tokens it multiplies (a multiple of 32; the ragged token tile has fewer).
+// A tile: its row pair, first token, the tokens it multiplies (a multiple of 32; the ragged token tile has fewer) and those of
+// them that exist; with sets, its set.
 struct PTile {
-  int pair, tok0, n;
+  int pair, tok0, n, toks, set;
 };
 __device__ __forceinline__ PTile tile_of(const PrefillParams& p, int tile) {
   const int nfull = p.pairs * p.full_tt;
@@ -152,9 +168,65 @@ __device__ __forceinline__ PTile tile_of(const PrefillParams& p, int tile) {
     t.tok0 = p.full_tt * p.tn;
     t.n = (p.M - t.tok0 + 31) & ~31;
   }
+  t.toks = min(t.n, p.M - t.tok0);
+  t.set = 0;
   return t;
 }
 
+// Sets: their slots and the tiles in front of each, in shared memory. A set's tokens are cut into equal tiles (a multiple of 32, at
+// most TN): up to some 160 tokens a tile costs its expansion, whatever it multiplies.
+struct SetTable {
+  const int2* bounds;
+  const int* first;  // [sets + 1]
+};
+// A role's walk over the tiles of its cluster; `set` moves on only.
+template <int MODE>
+__device__ __forceinline__ PTile walk_tile(const PrefillParams& p, int tile, int& set, const SetTable& tab) {
+  if constexpr (MODE != kSets) return tile_of(p, tile);
+  while (set + 1 < p.call.sets && tile >= tab.first[set + 1]) ++set;
+  const int2 b = tab.bounds[set];
+  const int n = b.y - b.x, tt = (n + p.tn - 1) / p.tn, per = ((n + tt - 1) / tt + 31) & ~31;
+  const int at = tile - tab.first[set];
+  PTile t;
+  t.set = set;
+  t.pair = at / tt;
+  const int c = (at - t.pair * tt) * per;
+  t.tok0 = b.x + c;
+  t.toks = min(per, n - c);
+  t.n = (t.toks + 31) & ~31;
+  return t;
+}
+
+// Four rows of a token with their sums complete: bias, activation, residual and the stores (dense layers).
+__device__ __forceinline__ void finish_four(const RaggedCall& c, int N, int tok, int r, const float4& acc) {
+  float v[4] = {acc.x, acc.y, acc.z, acc.w};
+  if (c.bias)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] += bf16_bits_to_float(c.bias[bias_index(r + i, N, c.act)]);
+  const bool gated = c.act == W4A16_ACT_SWIGLU;
+  const size_t o = static_cast<size_t>(tok) * c.ny + (gated ? r >> 1 : r);
+  if (gated) {
+    v[0] = logistic_times(v[0], v[0]) * v[1];
+    v[1] = logistic_times(v[2], v[2]) * v[3];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = activate(v[i], c.act);
+  }
+  const int n2 = gated ? 1 : 2;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (i < n2) {
+      if (c.residual) {
+        const uint32_t r2 = *reinterpret_cast<const uint32_t*>(c.residual + o + 2 * i);
+        v[2 * i] += bf16_bits_to_float(static_cast<uint16_t>(r2));
+        v[2 * i + 1] += bf16_bits_to_float(static_cast<uint16_t>(r2 >> 16));
+      }
+      *reinterpret_cast<uint32_t*>(c.y + o + 2 * i) =
+          float_to_bf16_bits(v[2 * i]) | (static_cast<uint32_t>(float_to_bf16_bits(v[2 * i + 1])) << 16);
+    }
+}
+
+template <int MODE>
 __global__ void __launch_bounds__(kPWarps * 32, 1) k_prefill(const __grid_constant__ PrefillParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -203,6 +275,36 @@ __global__ void __launch_bounds__(kPWarps * 32, 1) k_prefill(const __grid_consta
   const uint32_t tmem = *tmem_slot;
   const uint32_t tmem_a = tmem + (p.tn <= 128 ? 128 : 256);
 
+  int tiles = p.tiles, set = 0;
+  SetTable tab = {};
+  if constexpr (MODE == kSets) {
+    // the sets' bounds come from the kernel in front, and with them everything else
+    int2* bounds = reinterpret_cast<int2*>(tmem_slot + 2);
+    int* first = reinterpret_cast<int*>(bounds + p.call.sets);
+    tab.bounds = bounds;
+    tab.first = first;
+    pdl_wait();
+    if (warp == 0) {
+      int run = 0;
+      for (int e0 = 0; e0 < p.call.sets; e0 += 32) {
+        const int e = e0 + lane;
+        int2 b = make_int2(0, 0);
+        if (e < p.call.sets) bounds[e] = b = set_slots(p.call.offsets, e, p.call.slots);
+        const int mine = (b.y - b.x + p.tn - 1) / p.tn * p.pairs;
+        int upto = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+          const int v = __shfl_up_sync(0xffffffffu, upto, d);
+          if (lane >= d) upto += v;
+        }
+        if (e < p.call.sets) first[e] = run + upto - mine;
+        run += __shfl_sync(0xffffffffu, upto, 31);
+      }
+      if (lane == 0) first[p.call.sets] = run;
+    }
+    __syncthreads();
+    tiles = first[p.call.sets];
+  }
   const int cluster = blockIdx.x / (2 * S), nclusters = gridDim.x / (2 * S);
   const int g0 = p.G * split / S, g1 = p.G * (split + 1) / S;  // this split's k groups (S <= G)
   bool dead = false;
@@ -212,9 +314,11 @@ __global__ void __launch_bounds__(kPWarps * 32, 1) k_prefill(const __grid_consta
     if (lane == 0) {
       int st = 0;
       uint32_t ph = 1;
-      for (int tile = cluster; !dead && tile < p.tiles; tile += nclusters) {
-        const int rt = min(2 * tile_of(p, tile).pair + half, p.row_tiles - 1);
+      for (int tile = cluster; !dead && tile < tiles; tile += nclusters) {
+        const PTile t = walk_tile<MODE>(p, tile, set, tab);
+        const int rt = min(2 * t.pair + half, p.row_tiles - 1);
         const uint8_t* src = p.stream + (static_cast<size_t>(rt) * p.G + g0) * kTileGroupBytes;
+        if constexpr (MODE == kSets) src += p.call.set_bytes * t.set;
         for (int g = g0; g < g1; ++g, src += kTileGroupBytes) {
           if (!mbar_wait_bounded_relaxed(wempty_a + st * 8, ph, kPSpin)) {
             atomicExch(p.status, W4A16_ETIMEOUT);
@@ -242,8 +346,8 @@ __global__ void __launch_bounds__(kPWarps * 32, 1) k_prefill(const __grid_consta
       const uint32_t x16 = static_cast<uint32_t>(xbytes) >> 4;
       uint32_t j = 0, aph = 0, dph = 1;
       int a = 0;
-      for (int tile = cluster; !dead && tile < p.tiles; tile += nclusters, dph ^= 1) {
-        const uint32_t idesc = umma_idesc_bf16(kPRows, tile_of(p, tile).n);
+      for (int tile = cluster; !dead && tile < tiles; tile += nclusters, dph ^= 1) {
+        const uint32_t idesc = umma_idesc_bf16(kPRows, walk_tile<MODE>(p, tile, set, tab).n);
         if (!warp_agrees(mbar_wait_bounded(dempty_a, dph, kPSpin))) dead = true;  // (passes on the first tile)
         for (int g = g0; !dead && g < g1; ++g, ++j) {
           const uint32_t st = j & (kPSteps - 1);
@@ -276,7 +380,45 @@ __global__ void __launch_bounds__(kPWarps * 32, 1) k_prefill(const __grid_consta
     // ================================================================ activation producer
     // Two tiled TMA loads per k group (64 k each) into this CTA's half of the token tile; rows past M are zero-filled. The
     // leader's barrier expects both CTAs' bytes.
-    if (lane == 0) {
+    if (MODE == kSets) {
+      // Rows are gathered: a lane brings in four tokens of this CTA's half, in two loads per k group. Places past the tile's tokens
+      // repeat the last one.
+      const uint32_t xfull_l = map_to_rank(xfull_a, leader);
+      uint32_t j = 0;
+      for (int tile = cluster; !dead && tile < tiles; tile += nclusters) {
+        const PTile t = walk_tile<MODE>(p, tile, set, tab);
+        const bool mine = lane < t.n / 8;
+        int rows[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int slot = t.tok0 + min(half * (t.n >> 1) + 4 * lane + i, t.toks - 1);
+          const int row = p.call.x_rows ? __ldcg(p.call.x_rows + slot) : slot;
+          rows[i] = min(max(row, 0), p.call.x_tokens - 1);  // (no read outside x, whatever the rows hold)
+        }
+        const int4 r4 = make_int4(rows[0], rows[1], rows[2], rows[3]);
+        for (int g = g0; g < g1; ++g, ++j) {
+          const uint32_t st = j & (kPSteps - 1);
+          const uint32_t jd = j - kPSteps;
+          if (!warp_agrees(j < kPSteps || mbar_wait_bounded_relaxed(done_a + (jd & (kPDone - 1)) * 8, (jd / kPDone) & 1u, kPSpin))) {
+            dead = true;
+            break;
+          }
+          if (half == 0 && lane == 0) mbar_expect_tx(xfull_a + st * 8, t.n * 256);
+          __syncwarp();
+          if (mine) {
+            const uint32_t dst = xbuf_a + st * xbytes + lane * 512;
+            tma_gather_pair(dst, &p.amap, g * kGroup, r4, xfull_l + st * 8);
+            tma_gather_pair(dst + (xbytes >> 1), &p.amap, g * kGroup + 64, r4, xfull_l + st * 8);
+          }
+        }
+      }
+      if (dead && lane == 0) atomicExch(p.status, W4A16_ETIMEOUT);
+      if (dead && half == 0) {
+        for (uint32_t i = j < kPSteps ? 0 : j - kPSteps; i < j; ++i)
+          mbar_wait_bounded_relaxed(xfull_a + (i & (kPSteps - 1)) * 8, (i / kPSteps) & 1u, 1u << 10);
+      }
+      __syncwarp();
+    } else if (lane == 0) {
       const uint32_t xfull_l = map_to_rank(xfull_a, leader);
       pdl_wait();  // the previous kernel produced the activations (the weights never depend on it)
       uint32_t j = 0;
@@ -314,7 +456,7 @@ __global__ void __launch_bounds__(kPWarps * 32, 1) k_prefill(const __grid_consta
     const int row = q * 32 + lane;
     const uint32_t a_t = tmem_a + (static_cast<uint32_t>(q * 32) << 16);
     const uint32_t afull_l = map_to_rank(afull_a, leader);
-    const int ntiles = cluster < p.tiles ? (p.tiles - 1 - cluster) / nclusters + 1 : 0;
+    const int ntiles = cluster < tiles ? (tiles - 1 - cluster) / nclusters + 1 : 0;
     const uint32_t ngroups = static_cast<uint32_t>(ntiles) * static_cast<uint32_t>(g1 - g0);
     const uint32_t off_e = weight_slot(row, 0) * 16, off_o = kChunkBytes + weight_slot(row, 1) * 16;  // even and odd 32-k chunks
     int st = team, a = team;  // weight stage and A slot
@@ -411,9 +553,78 @@ __global__ void __launch_bounds__(kPWarps * 32, 1) k_prefill(const __grid_consta
     const uint32_t lane_t = tmem + (static_cast<uint32_t>(q * 32) << 16);
     const uint32_t dempty_l = map_to_rank(dempty_a, leader);
     uint32_t dph = 0;
-    for (int tile = cluster; tile < p.tiles; tile += nclusters, dph ^= 1) {
-      const PTile t = tile_of(p, tile);
+    // Layers with an epilogue: the sums are finished in registers on their way out, in fp32. The residual's tile waits in the
+    // staging buffer by then, brought in beside the main loop.
+    auto finish_tile = [&](const PTile& t, uint32_t phase) {
+      const RaggedCall& c = p.call;
+      const bool gated = c.act == W4A16_ACT_SWIGLU;
+      const int w8 = gated ? 3 : 4;                              // log2 of the eights of columns per token
+      const int r0 = (2 * t.pair + half) * kTileRows;
+      const int cols = min(kTileRows, p.N - r0) >> (gated ? 1 : 0);  // (<= 0: an odd last row tile's second half)
+      const int col0 = gated ? r0 >> 1 : r0, cl = (et & ((1 << w8) - 1)) * 8;
       uint16_t* cs = reinterpret_cast<uint16_t*>(cbuf);
+      const size_t line0 = static_cast<size_t>(t.tok0) * c.ny + col0 + cl;
+      if (c.residual) {
+        if (cl < cols)
+#pragma unroll 4
+          for (int m = et >> w8; m < t.toks; m += EW * 32 >> w8)
+            *reinterpret_cast<uint4*>(cs + (m << (w8 + 3)) + cl) = *reinterpret_cast<const uint4*>(c.residual + line0 + static_cast<size_t>(m) * c.ny);
+        named_bar_sync(1, EW * 32);
+      }
+      const int row = r0 + q * 32 + lane;
+      const float bias = c.bias && row < p.N
+                             ? bf16_bits_to_float(c.bias[static_cast<size_t>(t.set) * p.N + bias_index(row, p.N, c.act)]) : 0.f;
+      if (!dead && !warp_agrees(mbar_wait_bounded_relaxed(dfull_a, phase, kPSpin))) {
+        dead = true;
+        if (lane == 0) atomicExch(p.status, W4A16_ETIMEOUT);
+      }
+      if (!dead) {
+        tc_fence_after();
+        for (int m = eh * 16; m < t.n; m += EW / 4 * 16) {
+          float v[16];
+          tmem_ld<16>(lane_t + m, v);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] += bias;
+          if (gated) {
+            // gate and up are neighbouring lanes: each finishes eight of the pair's sixteen tokens
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float got = __shfl_xor_sync(0xffffffffu, lane & 1 ? v[i] : v[i + 8], 1);
+              const float gate = lane & 1 ? got : v[i], up = lane & 1 ? v[i + 8] : got;
+              uint16_t* at = cs + (m + i + (lane & 1) * 8) * (kTileRows / 2) + q * 16 + (lane >> 1);
+              float o = logistic_times(gate, gate) * up;
+              if (c.residual) o += bf16_bits_to_float(*at);
+              *at = float_to_bf16_bits(o);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              uint16_t* at = cs + (m + i) * kTileRows + q * 32 + lane;
+              float o = activate(v[i], c.act);
+              if (c.residual) o += bf16_bits_to_float(*at);
+              *at = float_to_bf16_bits(o);
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(dempty_l);
+      }
+      named_bar_sync(1, EW * 32);  // every epilogue warp comes here for every tile, dead or not
+      if (cl < cols && !dead)
+        for (int m = et >> w8; m < t.toks; m += EW * 32 >> w8)
+          *reinterpret_cast<uint4*>(c.y + line0 + static_cast<size_t>(m) * c.ny) = *reinterpret_cast<const uint4*>(cs + (m << (w8 + 3)) + cl);
+      named_bar_sync(1, EW * 32);  // the next tile overwrites the staged one
+    };
+    if constexpr (MODE != kPlain) pdl_wait();  // bias and residual may come from the kernel in front
+    for (int tile = cluster; tile < tiles; tile += nclusters, dph ^= 1) {
+      const PTile t = walk_tile<MODE>(p, tile, set, tab);
+      uint16_t* cs = reinterpret_cast<uint16_t*>(cbuf);
+      if constexpr (MODE != kPlain) {
+        finish_tile(t, dph);
+        continue;
+      }
       if (!dead && !warp_agrees(mbar_wait_bounded_relaxed(dfull_a, dph, kPSpin))) {
         dead = true;
         if (lane == 0) atomicExch(p.status, W4A16_ETIMEOUT);
@@ -460,7 +671,7 @@ __global__ void __launch_bounds__(kPWarps * 32, 1) k_prefill(const __grid_consta
     }
   }
 
-  if (S > 1) {
+  if (MODE != kSets && S > 1) {
     // ================================================================ split K: one tile per cluster
     // Every split's fp32 tile goes to its own shared memory (the activation stages: all MMAs have read them, and
     // [TN tokens][128 rows] floats are exactly their size), then split s adds up and stores the s-th share
@@ -486,6 +697,7 @@ __global__ void __launch_bounds__(kPWarps * 32, 1) k_prefill(const __grid_consta
     }
     __syncwarp();
     cluster_sync();
+    if constexpr (MODE != kPlain) pdl_wait();  // bias and residual may come from the kernel in front
     if (warp < PW + EW) {
       // Four rows of a token per thread: 16-byte loads from every split's tile, 256 contiguous bytes of C per warp. (One row per
       // thread, 4-byte loads and 64-byte runs of C took 1.6 us of a 5120 x 6144 launch at M = 77. The four layers of a block at M = 77,
@@ -512,6 +724,10 @@ __global__ void __launch_bounds__(kPWarps * 32, 1) k_prefill(const __grid_consta
             acc.z += part[s].z;
             acc.w += part[s].w;
           }
+        if constexpr (MODE != kPlain) {
+          if (r < p.N && tok < p.M) finish_four(p.call, p.N, tok, r, acc);
+          continue;
+        }
         if (r < p.N && tok < p.M) {  // (N is a multiple of 16)
           const size_t o = static_cast<size_t>(tok) * p.ldc + p.col0 + r;
           const uint2 v = make_uint2(float_to_bf16_bits(acc.x) | (static_cast<uint32_t>(float_to_bf16_bits(acc.y)) << 16),
@@ -608,6 +824,8 @@ PrefillPlan plan_prefill(int M, int pairs, int G, const int* device_clusters, in
   return best;
 }
 
+int table_bytes(int sets) { return sets * 12 + 16; }
+
 }  // namespace
 }  // namespace w4a16
 
@@ -635,6 +853,9 @@ int w4a16_workspace_free(w4a16_workspace_t* ws) {
   return W4A16_OK;
 }
 
+}  // extern "C"
+
+namespace w4a16 {
 namespace {
 void cluster_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* at, int splits, int clusters, int smem) {
   cfg.gridDim = dim3(2 * splits * clusters);
@@ -650,6 +871,7 @@ void cluster_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* at, int splits
 
 // How many clusters of 2 S CTAs (one CTA per SM) the device runs at once, index S; asked for once per device.
 // The kernel's shared-memory attribute is set on the way. Returns nullptr (and sets the error) on failure.
+template <int MODE>
 const int* cluster_slots(int dev, const DeviceInfo* di) {
   struct Slots {
     bool ready = false;
@@ -660,12 +882,12 @@ const int* cluster_slots(int dev, const DeviceInfo* di) {
   std::lock_guard<std::mutex> lk(mu);
   Slots& s = all[dev & 63];
   if (!s.ready) {
-    cudaError_t e = cudaFuncSetAttribute(k_prefill, cudaFuncAttributeMaxDynamicSharedMemorySize, di->smem_optin);
+    cudaError_t e = cudaFuncSetAttribute(k_prefill<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, di->smem_optin);
     for (int S = 1; S <= kPMaxSplit && e == cudaSuccess; ++S) {
       cudaLaunchConfig_t cfg = {};
       cudaLaunchAttribute at[1];
       cluster_config(cfg, at, S, 1, prefill_smem(kPMaxTN, kPTeams));
-      e = cudaOccupancyMaxActiveClusters(&s.n[S], k_prefill, &cfg);
+      e = cudaOccupancyMaxActiveClusters(&s.n[S], k_prefill<MODE>, &cfg);
     }
     if (e != cudaSuccess || s.n[1] < 1) {
       fail(W4A16_ECUDA, "gemm_prefill: the device runs no CTA pair of the kernel (%s)", cudaGetErrorString(e));
@@ -679,16 +901,61 @@ const int* cluster_slots(int dev, const DeviceInfo* di) {
 // The current device's plan for M tokens through `row_tiles` row tiles and G k groups of a layer of `layer_tiles` row
 // tiles. A shard is split as the whole layer would be, so that a row has the same bits sharded and unsharded; as its
 // tiles are fewer, they always fit the clusters that the layer's would. (What the shard's own choice would save is left.)
+template <int MODE>
 int current_plan(PrefillPlan& plan, int M, int row_tiles, int layer_tiles, int G) {
   const DeviceInfo* di = device_info();
   if (!di) return W4A16_ECUDA;
-  const int* slots = cluster_slots(di->device, di);
+  const int* slots = cluster_slots<MODE>(di->device, di);
   if (!slots) return W4A16_ECUDA;
   plan = plan_prefill(M, (layer_tiles + 1) / 2, G, slots, di->smem_optin, 0);
   if (row_tiles < layer_tiles && plan.tn > 0)
     plan = plan_prefill(M, (row_tiles + 1) / 2, G, slots, di->smem_optin, plan.splits);
   W4_REQUIRE(plan.tn > 0, "gemm_prefill: no launch shape for M = %d, %d row tiles x %d k groups", M, row_tiles, G);
   return W4A16_OK;
+}
+
+// The tensor map of activations [tokens][K]: boxes of 64 k x `rows` tokens, 128-byte swizzle, zeros past the last token.
+int encode_acts(CUtensorMap* map, const uint16_t* A, int K, int tokens, int rows) {
+  // driver entry point for the tensor-map encoder (no link-time dependency on libcuda)
+  typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                               const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                               CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static EncodeFn encode = nullptr;
+  if (!encode) {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult qres;
+    W4_CUDA(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &qres));
+    W4_REQUIRE(fn != nullptr && qres == cudaDriverEntryPointSuccess, "gemm_prefill: cuTensorMapEncodeTiled unavailable");
+    encode = reinterpret_cast<EncodeFn>(fn);
+  }
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(K), static_cast<cuuint64_t>(tokens)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(K) * 2};
+  const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(rows)};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUresult cr = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<uint16_t*>(A), dims, strides,
+                             box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return cr == CUDA_SUCCESS ? W4A16_OK : fail(W4A16_ECUDA, "gemm_prefill: cuTensorMapEncodeTiled failed (%d)", int(cr));
+}
+
+// The launch, programmatic unless a weight write is in front of a kernel that reads weights before its wait.
+template <int MODE>
+int enqueue_prefill(const PrefillParams& p, const PrefillPlan& plan, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[2];
+  cluster_config(cfg, at, plan.splits, plan.clusters, plan.smem);
+  const bool behind_write = MODE != kSets && take_weight_write(stream);
+  if (!behind_write && pdl_enabled()) {
+    // (behind a weight write the launch is fully ordered: the weights are read before the wait)
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 2;
+  }
+  cfg.stream = stream;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, k_prefill<MODE>, p);
+  if (e == cudaSuccess) return W4A16_OK;
+  if (behind_write) note_weight_write(stream);
+  return fail(W4A16_ECUDA, "gemm_prefill: launch: %s", cudaGetErrorString(e));
 }
 
 int launch_prefill(PrefillParams& p, uint16_t* C, const w4a16_weights_t* w, const uint16_t* A, int M, w4a16_workspace_t* ws,
@@ -710,7 +977,7 @@ int launch_prefill(PrefillParams& p, uint16_t* C, const w4a16_weights_t* w, cons
   p.pairs = (p.row_tiles + 1) / 2;
   PrefillPlan plan;
   const int layer_tiles = static_cast<int>((p.ldc + kTileRows - 1) / kTileRows);
-  if (int rc = current_plan(plan, M, p.row_tiles, layer_tiles, p.G)) return rc;
+  if (int rc = current_plan<kPlain>(plan, M, p.row_tiles, layer_tiles, p.G)) return rc;
   p.tn = plan.tn;
   p.splits = plan.splits;
   p.wdepth = plan.wdepth;
@@ -720,45 +987,50 @@ int launch_prefill(PrefillParams& p, uint16_t* C, const w4a16_weights_t* w, cons
   p.wide = (reinterpret_cast<uintptr_t>(C) & 15) == 0 && p.ldc % 8 == 0 && p.col0 % 8 == 0;
   for (int q = 0; q < p.npeers; ++q)
     if (reinterpret_cast<uintptr_t>(p.C_peers[q]) & 15) p.wide = 0;
-  {
-    // driver entry point for the tensor-map encoder (no link-time dependency on libcuda)
-    typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-    static EncodeFn encode = nullptr;
-    if (!encode) {
-      void* fn = nullptr;
-      cudaDriverEntryPointQueryResult qres;
-      W4_CUDA(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &qres));
-      W4_REQUIRE(fn != nullptr && qres == cudaDriverEntryPointSuccess, "gemm_prefill: cuTensorMapEncodeTiled unavailable");
-      encode = reinterpret_cast<EncodeFn>(fn);
-    }
-    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(w->in_f), static_cast<cuuint64_t>(M)};
-    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(w->in_f) * 2};
-    const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(plan.tn / 2)};
-    const cuuint32_t estr[2] = {1, 1};
-    const CUresult cr = encode(&p.amap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<uint16_t*>(A), dims, strides,
-                               box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (cr != CUDA_SUCCESS) return fail(W4A16_ECUDA, "gemm_prefill: cuTensorMapEncodeTiled failed (%d)", int(cr));
-  }
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute at[2];
-  cluster_config(cfg, at, plan.splits, plan.clusters, plan.smem);
-  const bool behind_write = take_weight_write(static_cast<cudaStream_t>(stream));
-  if (!behind_write && pdl_enabled()) {
-    // (behind a weight write the launch is fully ordered: the weights are read before the wait)
-    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.numAttrs = 2;
-  }
-  cfg.stream = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, k_prefill, p);
-  if (e == cudaSuccess) return W4A16_OK;
-  if (behind_write) note_weight_write(static_cast<cudaStream_t>(stream));
-  return fail(W4A16_ECUDA, "gemm_prefill: launch: %s", cudaGetErrorString(e));
+  if (int rc = encode_acts(&p.amap, A, w->in_f, M, plan.tn / 2)) return rc;
+  return enqueue_prefill<kPlain>(p, plan, static_cast<cudaStream_t>(stream));
 }
 }  // namespace
+
+int launch_prefill_ragged(const RaggedCall& c, cudaStream_t stream) {
+  const DeviceInfo* di = device_info();
+  if (!di) return W4A16_ECUDA;
+  PrefillParams p = {};
+  p.call = c;
+  p.stream = c.stream;
+  p.M = c.slots;
+  p.N = c.N;
+  p.K = c.K;
+  p.G = c.G;
+  p.row_tiles = (c.N + kTileRows - 1) / kTileRows;
+  p.pairs = (p.row_tiles + 1) / 2;
+  p.status = di->status;
+  PrefillPlan plan;
+  if (c.offsets == nullptr) {
+    if (int rc = current_plan<kDense>(plan, c.slots, p.row_tiles, p.row_tiles, c.G)) return rc;
+  } else {
+    const int* slots = cluster_slots<kSets>(di->device, di);
+    if (!slots) return W4A16_ECUDA;
+    // Tiles that hold the mean set with room for the larger ones
+    const long long want = (static_cast<long long>(c.slots) * 5 / 4 / c.sets + 31) / 32 * 32;
+    plan.tn = static_cast<int>(want < 64 ? 64 : want > kPSetsTN ? kPSetsTN : want);
+    plan.clusters = slots[1];
+    plan.wdepth = kPMaxWD;
+    while (plan.wdepth > kPTeams && prefill_smem(plan.tn, plan.wdepth) + table_bytes(c.sets) > di->smem_optin) plan.wdepth -= kPTeams;
+    plan.smem = prefill_smem(plan.tn, plan.wdepth) + table_bytes(c.sets);
+    W4_REQUIRE(plan.smem <= di->smem_optin, "experts_linear: %d bytes of shared memory", plan.smem);
+  }
+  p.tn = plan.tn;
+  p.splits = plan.splits;
+  p.wdepth = plan.wdepth;
+  p.full_tt = plan.full_tt;
+  p.tiles = plan.tiles;
+  if (int rc = encode_acts(&p.amap, c.x, c.K, c.x_tokens, c.offsets ? 1 : plan.tn / 2)) return rc;
+  return c.offsets ? enqueue_prefill<kSets>(p, plan, stream) : enqueue_prefill<kDense>(p, plan, stream);
+}
+}  // namespace w4a16
+
+extern "C" {
 
 int w4a16_gemm_prefill(uint16_t* C, const w4a16_weights_t* w, const uint16_t* A, int M, w4a16_workspace_t* ws,
                        void* stream) {
@@ -773,7 +1045,7 @@ int w4a16_prefill_plan(int M, int out_f, int in_f, int* tokens_per_tile, int* k_
              "prefill_plan: M = %d, %d x %d", M, out_f, in_f);
   PrefillPlan plan;
   const int row_tiles = (out_f + kTileRows - 1) / kTileRows;
-  if (int rc = current_plan(plan, M, row_tiles, row_tiles, in_f / kGroup)) return rc;
+  if (int rc = current_plan<kPlain>(plan, M, row_tiles, row_tiles, in_f / kGroup)) return rc;
   *tokens_per_tile = plan.tn;
   *k_splits = plan.splits;
   return W4A16_OK;

@@ -337,6 +337,8 @@ int run_ragged(RaggedCall& c, const char* who, cudaStream_t st) {
   p.c = c;
   p.row_tiles = (c.N + kTileRows - 1) / kTileRows;
   p.status = di->status;
+  // Many tokens per set: whole tiles on tcgen05
+  if (c.sets == 1 && c.offsets == nullptr ? c.slots > 32 : c.slots > 32LL * c.sets) return launch_prefill_ragged(c, st);
   // chunks of NT tokens at most: every set with tokens has one more than its whole ones
   const int used = c.slots < c.sets ? c.slots : c.sets;
   const int mean = (c.slots + c.sets - 1) / c.sets;

@@ -22,6 +22,9 @@ struct RaggedCall {
   int ny;                    // N, or N / 2 with the gated activation
 };
 
+// The prefill kernel on a checked call (prefill.cu).
+int launch_prefill_ragged(const RaggedCall& c, cudaStream_t stream);
+
 #ifdef __CUDACC__
 // v / (1 + exp(-v)); the gated and the tanh form come back to it: 0.5 v (1 + tanh u) = v / (1 + exp(-2 u)) holds its precision where
 // the tanh is near -1. Two special-function instructions a value.
