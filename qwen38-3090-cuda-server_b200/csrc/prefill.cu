@@ -52,6 +52,7 @@ constexpr int PW = 16;                      // dequant warps: 4 TMEM lane quarte
 constexpr int EW = 8;                       // epilogue warps: two per lane quarter, each half of the tokens
 constexpr int kWEpi0 = PW, kWWeights = PW + EW, kWIssue = kWWeights + 1, kWActs = kWIssue + 1;
 constexpr int kPWarps = kWActs + 1;
+constexpr int kPGather = 3;                 // with sets: warps that gather rows, kWActs and the ones behind it
 constexpr int kPRows = 2 * kTileRows;       // output rows of a CTA pair's tile
 constexpr int kPMaxTN = 256;                // tokens of a tile: a multiple of 32 (the pair's MMA needs N % 32 == 0)
 constexpr int kPMaxSplit = 4;               // 2 S <= 8 CTAs: the portable cluster size
@@ -66,7 +67,7 @@ constexpr int kPMaxA = 6;                   // A slots, at most
 constexpr int kPBars = 2 * kPMaxWD + kPDone + kPMaxA + kPSteps + 2;
 // Tensor memory: the accumulator's TN columns, the rest are slots of the A operand, 64 columns per k group.
 __host__ __device__ constexpr int a_slots(int tn) { return tn <= 128 ? 6 : 4; }
-constexpr int kPSetsTN = 224;               // with sets: their table needs the room that 256 tokens take
+constexpr int kPSetsTN = 160;               // tokens of a tile with sets
 static_assert(128 + 6 * 64 <= 512 && 256 + 4 * 64 <= 512 && kPMaxA <= kPDone && kPSteps <= kPDone, "ring depths");
 
 struct PrefillParams {
@@ -93,6 +94,7 @@ struct PrefillParams {
 // What an instance of the kernel does: the plain GEMM, a dense layer with bias, activation and residual in its epilogue, or
 // the same per set of tokens with its own weights (experts), rows gathered in the load.
 constexpr int kPlain = 0, kDense = 1, kSets = 2;
+__host__ __device__ constexpr int prefill_warps(int mode) { return mode == kSets ? kPWarps + kPGather - 1 : kPWarps; }
 
 __device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t d;
@@ -197,6 +199,47 @@ __device__ __forceinline__ PTile walk_tile(const PrefillParams& p, int tile, int
   return t;
 }
 
+// An epilogue warp's share of a finished tile: 32 rows (a thread each), every other sixteen of its n tokens, from tensor memory into the
+// staging buffer [token][column] with bias, activation and residual (which waits there) in fp32.
+template <int ACT, bool RES>
+__device__ __forceinline__ void read_out_tokens(uint16_t* cs, uint32_t lane_t, int n, int eh, int q, int lane, float bias) {
+#pragma unroll 2
+  for (int m = eh * 16; m < n; m += EW / 4 * 16) {
+    float v[16];
+    tmem_ld<16>(lane_t + m, v);
+    tmem_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] += bias;
+    if constexpr (ACT == W4A16_ACT_SWIGLU) {
+      // gate and up are neighbouring lanes: each finishes eight of the pair's sixteen tokens
+      uint16_t* at = cs + (m + (lane & 1) * 8) * (kTileRows / 2) + q * 16 + (lane >> 1);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float got = __shfl_xor_sync(0xffffffffu, lane & 1 ? v[i] : v[i + 8], 1);
+        const float gate = lane & 1 ? got : v[i], up = lane & 1 ? v[i + 8] : got;
+        float o = logistic_times(gate, gate) * up;
+        if constexpr (RES) o += bf16_bits_to_float(at[i * (kTileRows / 2)]);
+        at[i * (kTileRows / 2)] = float_to_bf16_bits(o);
+      }
+    } else {
+      uint16_t* at = cs + m * kTileRows + q * 32 + lane;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float o = activate<ACT>(v[i]);
+        if constexpr (RES) o += bf16_bits_to_float(at[i * kTileRows]);
+        at[i * kTileRows] = float_to_bf16_bits(o);
+      }
+    }
+  }
+}
+template <int MODE, int ACT>
+__device__ __forceinline__ void read_out(bool residual, uint16_t* cs, uint32_t lane_t, int n, int eh, int q, int lane, float bias) {
+  if (MODE == kDense && residual)  // (sets have none)
+    read_out_tokens<ACT, true>(cs, lane_t, n, eh, q, lane, bias);
+  else
+    read_out_tokens<ACT, false>(cs, lane_t, n, eh, q, lane, bias);
+}
+
 // Four rows of a token with their sums complete: bias, activation, residual and the stores (dense layers).
 __device__ __forceinline__ void finish_four(const RaggedCall& c, int N, int tok, int r, const float4& acc) {
   float v[4] = {acc.x, acc.y, acc.z, acc.w};
@@ -227,7 +270,7 @@ __device__ __forceinline__ void finish_four(const RaggedCall& c, int N, int tok,
 }
 
 template <int MODE>
-__global__ void __launch_bounds__(kPWarps * 32, 1) k_prefill(const __grid_constant__ PrefillParams p) {
+__global__ void __launch_bounds__(prefill_warps(MODE) * 32, 1) k_prefill(const __grid_constant__ PrefillParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int xbytes = p.tn * 128;  // one activation stage: two swizzled tiles of TN / 2 tokens x 64 k
@@ -258,6 +301,7 @@ __global__ void __launch_bounds__(kPWarps * 32, 1) k_prefill(const __grid_consta
       mbar_init(wempty_a + i * 8, 4);
     }
     for (int i = 0; i < kPDone; ++i) mbar_init(done_a + i * 8, 1);
+    // activations: one arrival that expects both CTAs' bytes; gathered rows: one arrival of each CTA
     for (int i = 0; i < kPSteps; ++i) mbar_init(xfull_a + i * 8, 1);
     for (int i = 0; i < kPMaxA; ++i) mbar_init(afull_a + i * 8, 8);
     mbar_init(dfull_a, 1);
@@ -279,7 +323,7 @@ __global__ void __launch_bounds__(kPWarps * 32, 1) k_prefill(const __grid_consta
   SetTable tab = {};
   if constexpr (MODE == kSets) {
     // the sets' bounds come from the kernel in front, and with them everything else
-    int2* bounds = reinterpret_cast<int2*>(tmem_slot + 2);
+    int2* bounds = reinterpret_cast<int2*>(bars + kPBars + 2 + kPGather * kPSetsTN / 4);  // (behind the gathering warps' lists of rows)
     int* first = reinterpret_cast<int*>(bounds + p.call.sets);
     tab.bounds = bounds;
     tab.first = first;
@@ -376,40 +420,47 @@ __global__ void __launch_bounds__(kPWarps * 32, 1) k_prefill(const __grid_consta
       }
       if (dead && lane == 0) atomicExch(p.status, W4A16_ETIMEOUT);
     }
-  } else if (warp == kWActs) {
+  } else if (warp == kWActs || (MODE == kSets && warp > kWActs)) {
     // ================================================================ activation producer
     // Two tiled TMA loads per k group (64 k each) into this CTA's half of the token tile; rows past M are zero-filled. The
     // leader's barrier expects both CTAs' bytes.
-    if (MODE == kSets) {
-      // Rows are gathered: a lane brings in four tokens of this CTA's half, in two loads per k group. Places past the tile's tokens
-      // repeat the last one.
+    if (MODE == kSets && p.call.x_rows) {
+      // Rows are gathered by TMA, four rows of 64 k a load, half of the tile's tokens in each CTA; places past the tile's tokens repeat
+      // the last one. Issuing a load takes a warp some 25 cycles and a group has up to 40, so three warps take the groups in turn, each with
+      // its own list of rows. 64 experts 2048 x 5120 of 8 picks, us at 300 / 1200 / 4096 tokens: one warp (a shuffle per row) 232 / 460 /
+      // 1270, two 178 / 319 / 831, with lists 145 / 267 / 675, three 140 / 245 / 623, four the same; rows already in slot order 133 / 216 / 548.
       const uint32_t xfull_l = map_to_rank(xfull_a, leader);
+      int* rows = reinterpret_cast<int*>(bars + kPBars + 2) + (warp - kWActs) * (kPSetsTN / 2);  // (16-byte aligned)
       uint32_t j = 0;
       for (int tile = cluster; !dead && tile < tiles; tile += nclusters) {
         const PTile t = walk_tile<MODE>(p, tile, set, tab);
-        const bool mine = lane < t.n / 8;
-        int rows[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int slot = t.tok0 + min(half * (t.n >> 1) + 4 * lane + i, t.toks - 1);
-          const int row = p.call.x_rows ? __ldcg(p.call.x_rows + slot) : slot;
-          rows[i] = min(max(row, 0), p.call.x_tokens - 1);  // (no read outside x, whatever the rows hold)
+        __syncwarp();
+        for (int i = lane; i < t.n >> 1; i += 32) {
+          const int slot = t.tok0 + min(half * (t.n >> 1) + i, t.toks - 1);
+          rows[i] = min(max(__ldcg(p.call.x_rows + slot), 0), p.call.x_tokens - 1);  // (no read outside x, whatever the rows hold)
         }
-        const int4 r4 = make_int4(rows[0], rows[1], rows[2], rows[3]);
+        __syncwarp();
+        const int fours = t.n / 8;
         for (int g = g0; g < g1; ++g, ++j) {
+          if (j % kPGather != static_cast<uint32_t>(warp - kWActs)) continue;
           const uint32_t st = j & (kPSteps - 1);
           const uint32_t jd = j - kPSteps;
-          if (!warp_agrees(j < kPSteps || mbar_wait_bounded_relaxed(done_a + (jd & (kPDone - 1)) * 8, (jd / kPDone) & 1u, kPSpin))) {
+          if (!warp_agrees(j < kPSteps || mbar_wait_bounded(done_a + (jd & (kPDone - 1)) * 8, (jd / kPDone) & 1u, kPSpin))) {
             dead = true;
             break;
           }
           if (half == 0 && lane == 0) mbar_expect_tx(xfull_a + st * 8, t.n * 256);
           __syncwarp();
-          if (mine) {
-            const uint32_t dst = xbuf_a + st * xbytes + lane * 512;
-            tma_gather_pair(dst, &p.amap, g * kGroup, r4, xfull_l + st * 8);
-            tma_gather_pair(dst + (xbytes >> 1), &p.amap, g * kGroup + 64, r4, xfull_l + st * 8);
+          const uint32_t dst = xbuf_a + st * xbytes;
+          if (elect_one()) {
+#pragma unroll 4
+            for (int i = 0; i < fours; ++i) {
+              const int4 rr = *reinterpret_cast<const int4*>(rows + 4 * i);
+              tma_gather_pair(dst + i * 512, &p.amap, g * kGroup, rr, xfull_l + st * 8);
+              tma_gather_pair(dst + i * 512 + (xbytes >> 1), &p.amap, g * kGroup + 64, rr, xfull_l + st * 8);
+            }
           }
+          __syncwarp();
         }
       }
       if (dead && lane == 0) atomicExch(p.status, W4A16_ETIMEOUT);
@@ -418,12 +469,12 @@ __global__ void __launch_bounds__(kPWarps * 32, 1) k_prefill(const __grid_consta
           mbar_wait_bounded_relaxed(xfull_a + (i & (kPSteps - 1)) * 8, (i / kPSteps) & 1u, 1u << 10);
       }
       __syncwarp();
-    } else if (lane == 0) {
+    } else if (warp == kWActs && lane == 0) {
       const uint32_t xfull_l = map_to_rank(xfull_a, leader);
       pdl_wait();  // the previous kernel produced the activations (the weights never depend on it)
       uint32_t j = 0;
-      for (int tile = cluster; !dead && tile < p.tiles; tile += nclusters) {
-        const PTile t = tile_of(p, tile);
+      for (int tile = cluster; !dead && tile < tiles; tile += nclusters) {
+        const PTile t = walk_tile<MODE>(p, tile, set, tab);
         const int y = t.tok0 + half * (t.n >> 1);
         for (int g = g0; g < g1; ++g, ++j) {
           const uint32_t st = j & (kPSteps - 1);
@@ -580,32 +631,12 @@ __global__ void __launch_bounds__(kPWarps * 32, 1) k_prefill(const __grid_consta
       }
       if (!dead) {
         tc_fence_after();
-        for (int m = eh * 16; m < t.n; m += EW / 4 * 16) {
-          float v[16];
-          tmem_ld<16>(lane_t + m, v);
-          tmem_wait_ld();
-#pragma unroll
-          for (int i = 0; i < 16; ++i) v[i] += bias;
-          if (gated) {
-            // gate and up are neighbouring lanes: each finishes eight of the pair's sixteen tokens
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float got = __shfl_xor_sync(0xffffffffu, lane & 1 ? v[i] : v[i + 8], 1);
-              const float gate = lane & 1 ? got : v[i], up = lane & 1 ? v[i + 8] : got;
-              uint16_t* at = cs + (m + i + (lane & 1) * 8) * (kTileRows / 2) + q * 16 + (lane >> 1);
-              float o = logistic_times(gate, gate) * up;
-              if (c.residual) o += bf16_bits_to_float(*at);
-              *at = float_to_bf16_bits(o);
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              uint16_t* at = cs + (m + i) * kTileRows + q * 32 + lane;
-              float o = activate(v[i], c.act);
-              if (c.residual) o += bf16_bits_to_float(*at);
-              *at = float_to_bf16_bits(o);
-            }
-          }
+        switch (c.act) {
+          case W4A16_ACT_SWIGLU: read_out<MODE, W4A16_ACT_SWIGLU>(c.residual, cs, lane_t, t.n, eh, q, lane, bias); break;
+          case W4A16_ACT_SILU: read_out<MODE, W4A16_ACT_SILU>(c.residual, cs, lane_t, t.n, eh, q, lane, bias); break;
+          case W4A16_ACT_GELU: read_out<MODE, W4A16_ACT_GELU>(c.residual, cs, lane_t, t.n, eh, q, lane, bias); break;
+          case W4A16_ACT_GELU_TANH: read_out<MODE, W4A16_ACT_GELU_TANH>(c.residual, cs, lane_t, t.n, eh, q, lane, bias); break;
+          default: read_out<MODE, W4A16_ACT_NONE>(c.residual, cs, lane_t, t.n, eh, q, lane, bias);
         }
         tc_fence_before();
         __syncwarp();
@@ -824,7 +855,7 @@ PrefillPlan plan_prefill(int M, int pairs, int G, const int* device_clusters, in
   return best;
 }
 
-int table_bytes(int sets) { return sets * 12 + 16; }
+int table_bytes(int sets) { return kPGather * (kPSetsTN / 2) * 4 + sets * 12 + 16; }
 
 }  // namespace
 }  // namespace w4a16
@@ -857,9 +888,9 @@ int w4a16_workspace_free(w4a16_workspace_t* ws) {
 
 namespace w4a16 {
 namespace {
-void cluster_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* at, int splits, int clusters, int smem) {
+void cluster_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* at, int warps, int splits, int clusters, int smem) {
   cfg.gridDim = dim3(2 * splits * clusters);
-  cfg.blockDim = dim3(kPWarps * 32);
+  cfg.blockDim = dim3(warps * 32);
   cfg.dynamicSmemBytes = smem;
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = 2 * splits;
@@ -886,7 +917,7 @@ const int* cluster_slots(int dev, const DeviceInfo* di) {
     for (int S = 1; S <= kPMaxSplit && e == cudaSuccess; ++S) {
       cudaLaunchConfig_t cfg = {};
       cudaLaunchAttribute at[1];
-      cluster_config(cfg, at, S, 1, prefill_smem(kPMaxTN, kPTeams));
+      cluster_config(cfg, at, prefill_warps(MODE), S, 1, prefill_smem(kPMaxTN, kPTeams));
       e = cudaOccupancyMaxActiveClusters(&s.n[S], k_prefill<MODE>, &cfg);
     }
     if (e != cudaSuccess || s.n[1] < 1) {
@@ -943,7 +974,7 @@ template <int MODE>
 int enqueue_prefill(const PrefillParams& p, const PrefillPlan& plan, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute at[2];
-  cluster_config(cfg, at, plan.splits, plan.clusters, plan.smem);
+  cluster_config(cfg, at, prefill_warps(MODE), plan.splits, plan.clusters, plan.smem);
   const bool behind_write = MODE != kSets && take_weight_write(stream);
   if (!behind_write && pdl_enabled()) {
     // (behind a weight write the launch is fully ordered: the weights are read before the wait)
@@ -1011,9 +1042,10 @@ int launch_prefill_ragged(const RaggedCall& c, cudaStream_t stream) {
   } else {
     const int* slots = cluster_slots<kSets>(di->device, di);
     if (!slots) return W4A16_ECUDA;
-    // Tiles that hold the mean set with room for the larger ones
-    const long long want = (static_cast<long long>(c.slots) * 5 / 4 / c.sets + 31) / 32 * 32;
-    plan.tn = static_cast<int>(want < 64 ? 64 : want > kPSetsTN ? kPSetsTN : want);
+    // Tiles of up to 160 tokens, whatever the sets' sizes: as wide as an expansion pays for (4 TN cycles against some 650), while
+    // sets of any size are cut evenly. 64 experts 2048 x 5120, rows in slot order, TN = 64 / 96 / 128 / 160 / 192 / 224: at 300 slots
+    // per 8 experts 155 / 144 / 140 / 131 / 131 / 133 us, at 4096 904 / 699 / 600 / 562 / 573 / 611.
+    plan.tn = kPSetsTN;
     plan.clusters = slots[1];
     plan.wdepth = kPMaxWD;
     while (plan.wdepth > kPTeams && prefill_smem(plan.tn, plan.wdepth) + table_bytes(c.sets) > di->smem_optin) plan.wdepth -= kPTeams;
@@ -1025,7 +1057,7 @@ int launch_prefill_ragged(const RaggedCall& c, cudaStream_t stream) {
   p.wdepth = plan.wdepth;
   p.full_tt = plan.full_tt;
   p.tiles = plan.tiles;
-  if (int rc = encode_acts(&p.amap, c.x, c.K, c.x_tokens, c.offsets ? 1 : plan.tn / 2)) return rc;
+  if (int rc = encode_acts(&p.amap, c.x, c.K, c.x_tokens, c.x_rows ? 1 : plan.tn / 2)) return rc;
   return c.offsets ? enqueue_prefill<kSets>(p, plan, stream) : enqueue_prefill<kDense>(p, plan, stream);
 }
 }  // namespace w4a16
