@@ -12,9 +12,10 @@
 //   * eight consumer warps take 32 rows x 64 k each: mma.sync m16n8k16 with the weights as the A operand straight from the
 //     expansion. The fragments' k order is free as long as both operands share it, so a lane takes 16 consecutive k of
 //     its row (8 bytes of codes) and of its token (two 16-byte loads).
-#include <atomic>
 #include <climits>
 #include <cstring>
+#include <mutex>
+#include <type_traits>
 
 #include "ragged.cuh"
 
@@ -22,10 +23,15 @@ namespace w4a16 {
 namespace {
 
 constexpr int kRCons = 8;                        // consumer warps
-constexpr int kRThreads = (kRCons + 1) * 32;
-constexpr int kRMaxDepth = 16;                   // ring stages at most
-constexpr int kXPitch = 272;                     // bytes of a token's 128 activations in a stage: 16 more than they are, against bank conflicts
+constexpr int kRThreads = (kRCons + 2) * 32;     // and a producer and a warp that prepares the rows' constants
+constexpr int kRMaxDepth = 8;                    // ring stages at most
+constexpr int kRMaxSplit = 8;                    // CTAs that share a unit at most: the portable cluster size
+constexpr int kRGroups = 2;                      // k groups of a stage
+constexpr int kXPitch = kRGroups * 256 + 16;     // bytes of a token's activations in a stage: 16 more than they are, against bank conflicts
 constexpr uint32_t kRSpin = 1u << 20;
+
+template <int N>
+using Const = std::integral_constant<int, N>;
 
 struct RaggedParams {
   RaggedCall c;
@@ -34,9 +40,58 @@ struct RaggedParams {
 };
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Shared-memory loads at a 32-bit address plus a constant (the address arithmetic of generic pointers would double it)
+template <int OFF>
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2 + %3];" : "=r"(v.x), "=r"(v.y) : "r"(a), "n"(OFF));
+  return v;
+}
+template <int OFF>
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4 + %5];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a), "n"(OFF));
+  return v;
+}
+template <int OFF>
+__device__ __forceinline__ uint32_t lds_u16(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u16 %0, [%1 + %2];" : "=r"(v) : "r"(a), "n"(OFF));
+  return v;
+}
+template <int OFF>
+__device__ __forceinline__ uint32_t lds_u8(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u8 %0, [%1 + %2];" : "=r"(v) : "r"(a), "n"(OFF));
+  return v;
+}
+
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ void sts32(uint32_t a, uint32_t v) { asm volatile("st.shared.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory"); }
+__device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+
+// (a & mask) | bits in one instruction; written as such the compiler takes two, as it has room for one constant in each
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t bits) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "r"(mask), "r"(bits));
+  return d;
+}
+
+__device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
 }
 
 // Where unit u of the launch lies: set, first slot, tokens, row tile. The chunks of one row tile are neighbours, so that its
@@ -57,13 +112,76 @@ __device__ __forceinline__ Unit unit_of(int u, int& e, const int* first, const i
   return t;
 }
 
+// A stage: the groups' weight blocks, the tokens' activations, then what the expansion needs of every row and group (16 bytes
+// each) and a word that says whether some scale is large.
+template <int NT>
+__host__ __device__ constexpr int consts_offset() {
+  return kRGroups * kTileGroupBytes + NT * kXPitch;
+}
+template <int NT>
+__host__ __device__ constexpr int large_offset() {
+  return consts_offset<NT>() + kRGroups * kTileRows * 16;
+}
 template <int NT>
 __host__ __device__ constexpr int stage_bytes() {
-  return kTileGroupBytes + NT * kXPitch;
+  return large_offset<NT>() + 16;
 }
 template <int NT>
 __host__ __device__ constexpr int sum_bytes() {  // the two k halves' sums: [2][NT tokens][128 rows] floats
   return 2 * NT * kTileRows * 4;
+}
+
+// bf16((q - z) s) of a word's eight weights, pairs of k, from a row's constants {128 + z, s, -z / 4, 4 s} (bf16 pairs). Nibbles 0 and 4
+// become (128 + q) - (128 + z) by one OR and a subtraction, exactly; nibbles 1 and 5 stay where they are: as a bf16 pair
+// w & 0x00F000F0 is q 2^-129, so one FMA makes (q - z) / 4 of it, exactly too, and 4 s is exact unless s is 2^126 or more: then
+// every nibble is shifted down. The product rounds once in either form.
+template <bool LARGE>
+__device__ __forceinline__ void expand_word(uint32_t word, const uint4& c, uint32_t (&a)[4]) {
+  const uint32_t w8 = word >> 8;
+  a[0] = mul_bf16x2(sub_bf16x2(and_or(word, 0x000F000Fu, 0x43004300u), c.x), c.y);
+  a[2] = mul_bf16x2(sub_bf16x2(and_or(w8, 0x000F000Fu, 0x43004300u), c.x), c.y);
+  if constexpr (LARGE) {
+    a[1] = mul_bf16x2(sub_bf16x2(and_or(word >> 4, 0x000F000Fu, 0x43004300u), c.x), c.y);
+    a[3] = mul_bf16x2(sub_bf16x2(and_or(w8 >> 4, 0x000F000Fu, 0x43004300u), c.x), c.y);
+  } else {
+    a[1] = mul_bf16x2(fma_bf16x2(word & 0x00F000F0u, 0x7F007F00u, c.z), c.w);
+    a[3] = mul_bf16x2(fma_bf16x2(w8 & 0x00F000F0u, 0x7F007F00u, c.z), c.w);
+  }
+}
+
+// A warp's 32 rows x 64 k of group I of a stage times the tokens: the lane's rows r0, + 8, + 16, + 24, 16 consecutive k of each.
+template <int NT, int I, bool LARGE>
+__device__ __forceinline__ void multiply_group(float (&acc)[2][NT / 8][4], uint32_t w_at, uint32_t w_last, uint32_t c_at, uint32_t x_at, int n) {
+  constexpr int W = I * kTileGroupBytes, X = I * 256, C = I * kTileRows * 16;
+  const uint2 w[4] = {lds64<W>(w_at), lds64<W + 128>(w_at), lds64<W + 256>(w_at), lds64<W>(w_last)};
+  const uint4 c[4] = {lds128<C>(c_at), lds128<C + 128>(c_at), lds128<C + 256>(c_at), lds128<C + 384>(c_at)};
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {  // 8 of the lane's 16 k: one word of codes, one 16-byte load per token
+    uint32_t a[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) expand_word<LARGE>(h ? w[i].y : w[i].x, c[i], a[i]);
+    auto tokens8 = [&](auto at) {
+      constexpr int j = decltype(at)::value;
+      const uint4 b = h ? lds128<X + 8 * j * kXPitch + 16>(x_at) : lds128<X + 8 * j * kXPitch>(x_at);
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        mma_bf16(acc[m][j], a[2 * m][0], a[2 * m + 1][0], a[2 * m][1], a[2 * m + 1][1], b.x, b.y);
+        mma_bf16(acc[m][j], a[2 * m][2], a[2 * m + 1][2], a[2 * m][3], a[2 * m + 1][3], b.z, b.w);
+      }
+    };
+    tokens8(Const<0>());
+    if constexpr (NT > 8)
+      if (n > 8) tokens8(Const<1>());
+    if constexpr (NT > 16) {
+      if (n > 16) tokens8(Const<2>());
+      if (n > 24) tokens8(Const<3>());
+    }
+  }
+}
+template <int NT, bool LARGE>
+__device__ __forceinline__ void multiply_stage(float (&acc)[2][NT / 8][4], uint32_t w_at, uint32_t w_last, uint32_t c_at, uint32_t x_at, int n, bool two) {
+  multiply_group<NT, 0, LARGE>(acc, w_at, w_last, c_at, x_at, n);
+  if (two) multiply_group<NT, 1, LARGE>(acc, w_at, w_last, c_at, x_at, n);
 }
 
 template <int NT>
@@ -73,18 +191,19 @@ __global__ void __launch_bounds__(kRThreads, 2) k_ragged(const __grid_constant__
   float* sums = reinterpret_cast<float*>(smem);
   uint8_t* ring = smem + sum_bytes<NT>();
   uint64_t* bars = reinterpret_cast<uint64_t*>(ring + p.depth * stage_bytes<NT>());
-  int2* bounds = reinterpret_cast<int2*>(bars + 2 * kRMaxDepth);
+  int2* bounds = reinterpret_cast<int2*>(bars + 3 * kRMaxDepth);
   int* first = reinterpret_cast<int*>(bounds + c.sets);  // [sets + 1] units in front of each set
 
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const int S = p.splits, split = S > 1 ? static_cast<int>(cluster_rank()) : 0;
   const int cluster = blockIdx.x / S, nclusters = gridDim.x / S;
-  const uint32_t ring_a = smem_u32(ring), full_a = smem_u32(bars), empty_a = full_a + kRMaxDepth * 8;
+  const uint32_t ring_a = smem_u32(ring), full_a = smem_u32(bars), empty_a = full_a + kRMaxDepth * 8, ready_a = empty_a + kRMaxDepth * 8;
   if (tid == 0) {
     for (int i = 0; i < p.depth; ++i) {
       mbar_init(full_a + i * 8, 1);
       mbar_init(empty_a + i * 8, kRCons);
+      mbar_init(ready_a + i * 8, 1);
     }
     fence_mbar_init();
   }
@@ -129,18 +248,18 @@ __global__ void __launch_bounds__(kRThreads, 2) k_ragged(const __grid_constant__
       if (c.x_rows) row = __ldcg(c.x_rows + row);
       row = min(max(row, 0), c.x_tokens - 1);  // (no read outside x, whatever the rows hold)
       const uint16_t* xr = c.x + static_cast<size_t>(row) * c.K + static_cast<size_t>(g0) * kGroup;
-      for (int g = g0; g < g1; ++g, src += kTileGroupBytes, xr += kGroup) {
+      for (int g = g0; g < g1; g += kRGroups, src += kRGroups * kTileGroupBytes, xr += kRGroups * kGroup) {
         if (!warp_agrees(mbar_wait_bounded_relaxed(empty_a + st * 8, ph, kRSpin))) {
           dead = true;
           break;
         }
-        const uint32_t dst = ring_a + st * stage_bytes<NT>();
+        const uint32_t dst = ring_a + st * stage_bytes<NT>(), ng = min(kRGroups, g1 - g);
         if (lane == 0) {
-          mbar_expect_tx(full_a + st * 8, kTileGroupBytes + t.n * kGroup * 2);
-          bulk_g2s(dst, src, kTileGroupBytes, full_a + st * 8);
+          mbar_expect_tx(full_a + st * 8, ng * (kTileGroupBytes + t.n * kGroup * 2));
+          bulk_g2s(dst, src, ng * kTileGroupBytes, full_a + st * 8);
         }
         __syncwarp();
-        if (lane < t.n) bulk_g2s(dst + kTileGroupBytes + lane * kXPitch, xr, kGroup * 2, full_a + st * 8);
+        if (lane < t.n) bulk_g2s(dst + kRGroups * kTileGroupBytes + lane * kXPitch, xr, ng * kGroup * 2, full_a + st * 8);
         ++issued;
         if (++st == p.depth) {
           st = 0;
@@ -160,53 +279,76 @@ __global__ void __launch_bounds__(kRThreads, 2) k_ragged(const __grid_constant__
     return;
   }
 
+  if (warp == kRCons + 1) {
+    // ================================================================ the rows' constants
+    // Every lane of eight consumer lanes needs the same ones: made once, read by 16-byte loads. 34816 x 5120 at M = 1
+    // MEASURED.
+    uint32_t ph = 0;
+    for (int u = cluster; !dead && u < units; u += nclusters) {
+      for (int g = g0; g < g1; g += kRGroups) {
+        if (!warp_agrees(mbar_wait_bounded(full_a + st * 8, ph, kRSpin))) {
+          dead = true;
+          break;
+        }
+        const uint32_t blk = ring_a + st * stage_bytes<NT>();
+        bool large = false;
+#pragma unroll
+        for (int i = 0; i < kRGroups; ++i) {  // (an odd last group's neighbour is whatever the stage held before)
+          const uint32_t at = blk + i * kTileGroupBytes, to = blk + consts_offset<NT>() + i * kTileRows * 16 + lane * 16;
+          const uint32_t sc[4] = {lds_u16<kTgScaleOff>(at + lane * 2), lds_u16<kTgScaleOff + 64>(at + lane * 2),
+                                  lds_u16<kTgScaleOff + 128>(at + lane * 2), lds_u16<kTgScaleOff + 192>(at + lane * 2)};
+          const uint32_t zp[4] = {lds_u8<kTgZpOff>(at + lane), lds_u8<kTgZpOff + 32>(at + lane), lds_u8<kTgZpOff + 64>(at + lane),
+                                  lds_u8<kTgZpOff + 96>(at + lane)};
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const uint32_t z = __byte_perm(zp[r], 0x43434343u, 0x4040), s2 = __byte_perm(sc[r], 0, 0x1010);  // (128 + z, 128 + z), (s, s)
+            sts128(to + r * 512, z, s2, fma_bf16x2(z, 0xBE80BE80u, 0x42004200u), mul_bf16x2(s2, 0x40804080u));  // -z / 4, 4 s
+            large |= (sc[r] & 0x7FFFu) - 0x7E80u < 0x100u;
+          }
+        }
+        large = __any_sync(0xffffffffu, large);
+        if (lane == 0) {
+          sts32(blk + large_offset<NT>(), large);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(ready_a + st * 8);
+        if (++st == p.depth) {
+          st = 0;
+          ph ^= 1;
+        }
+      }
+    }
+    if (dead && lane == 0) atomicExch(p.status, W4A16_ETIMEOUT);
+    __syncwarp();
+    if (S > 1) {
+      cluster_sync();
+      cluster_sync();
+    }
+    return;
+  }
+
   // ================================================================ consumers
   const int half = warp & 1, r0 = (warp >> 1) * 32 + (lane >> 2), t4 = lane & 3;
   const int chunk = 2 * half + (t4 >> 1);
-  const uint32_t w_off = chunk * kChunkBytes + (t4 & 1) * 8;
-  const uint32_t x_off = kTileGroupBytes + (lane >> 2) * kXPitch + (half * 64 + t4 * 16) * 2;
+  // Offsets of the lane's codes in a stage: rows r0, + 8, + 16 lie 128 bytes apart, the last may wrap round (weight_slot)
+  const uint32_t w_off = chunk * kChunkBytes + (t4 & 1) * 8 + weight_slot(r0, chunk) * 16;
+  const uint32_t w_last = chunk * kChunkBytes + (t4 & 1) * 8 + weight_slot(r0 + 24, chunk) * 16;
+  const uint32_t c_off = consts_offset<NT>() + r0 * 16;
+  const uint32_t x_off = kRGroups * kTileGroupBytes + (lane >> 2) * kXPitch + (half * 64 + t4 * 16) * 2;
   uint32_t ph = 0;
   for (int u = cluster; u < units; u += nclusters) {
     const Unit t = unit_of<NT>(u, e, first, bounds, c.sets);
     float acc[2][NT / 8][4] = {};
-    for (int g = g0; g < g1 && !dead; ++g) {
-      if (!warp_agrees(mbar_wait_bounded(full_a + st * 8, ph, kRSpin))) {
+    for (int g = g0; g < g1 && !dead; g += kRGroups) {
+      if (!warp_agrees(mbar_wait_bounded(ready_a + st * 8, ph, kRSpin))) {  // (behind the weights' and activations' arrival)
         dead = true;
         break;
       }
-      const uint8_t* blk = ring + st * stage_bytes<NT>();
-      uint2 w[4];
-      uint32_t zpair[4], spair[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = r0 + 8 * i;
-        w[i] = *reinterpret_cast<const uint2*>(blk + w_off + weight_slot(r, chunk) * 16);
-        const uint32_t sc = reinterpret_cast<const uint16_t*>(blk + kTgScaleOff)[r];
-        spair[i] = sc | (sc << 16);
-        zpair[i] = __byte_perm(blk[kTgZpOff + r], 0x43434343u, 0x4040);  // bf16 pair (128 + zp, 128 + zp)
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {  // 8 of the lane's 16 k: one word of codes, one 16-byte load per token
-        uint32_t a[4][4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t word = h ? w[i].y : w[i].x;
-#pragma unroll
-          for (int pp = 0; pp < 4; ++pp)  // (128 + q) - (128 + zp) is exact, the product rounds once
-            a[i][pp] = mul_bf16x2(sub_bf16x2(((word >> (4 * pp)) & 0x000F000Fu) | 0x43004300u, zpair[i]), spair[i]);
-        }
-#pragma unroll
-        for (int j = 0; j < NT / 8; ++j) {
-          if (j == 0 || 8 * j < t.n) {
-            const uint4 b = *reinterpret_cast<const uint4*>(blk + x_off + 8 * j * kXPitch + 16 * h);
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-              mma_bf16(acc[m][j], a[2 * m][0], a[2 * m + 1][0], a[2 * m][1], a[2 * m + 1][1], b.x, b.y);
-              mma_bf16(acc[m][j], a[2 * m][2], a[2 * m + 1][2], a[2 * m][3], a[2 * m + 1][3], b.z, b.w);
-            }
-          }
-        }
-      }
+      const uint32_t blk = ring_a + st * stage_bytes<NT>();
+      if (lds32(blk + large_offset<NT>()) == 0)
+        multiply_stage<NT, false>(acc, blk + w_off, blk + w_last, blk + c_off, blk + x_off, t.n, g + 1 < g1);
+      else
+        multiply_stage<NT, true>(acc, blk + w_off, blk + w_last, blk + c_off, blk + x_off, t.n, g + 1 < g1);
       __syncwarp();
       if (lane == 0) mbar_arrive(empty_a + st * 8);
       if (++st == p.depth) {
@@ -274,21 +416,61 @@ __global__ void __launch_bounds__(kRThreads, 2) k_ragged(const __grid_constant__
 }
 
 template <int NT>
+int fixed_bytes(int sets) {
+  return sum_bytes<NT>() + 3 * kRMaxDepth * 8 + sets * 8 + (sets + 1) * 4;
+}
+// How many clusters of n CTAs the device runs at once, index n; asked for once per device, with the largest shared memory that
+// leaves two CTAs per SM. The kernel's shared-memory attribute is set on the way.
+template <int NT>
+const int* clusters_at_once(const DeviceInfo* di) {
+  struct Fit {
+    bool ready = false;
+    int n[kRMaxSplit + 1] = {};
+  };
+  static std::mutex mu;
+  static Fit all[64];
+  std::lock_guard<std::mutex> lk(mu);
+  Fit& f = all[di->device & 63];
+  if (!f.ready) {
+    cudaError_t e = cudaFuncSetAttribute(k_ragged<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, di->smem_optin);
+    for (int n = 1; n <= kRMaxSplit && e == cudaSuccess; ++n) {
+      cudaLaunchConfig_t cfg = {};
+      cudaLaunchAttribute at[1];
+      cfg.gridDim = dim3(n);
+      cfg.blockDim = dim3(kRThreads);
+      cfg.dynamicSmemBytes = di->smem_per_sm / 2 - di->smem_reserved;
+      at[0].id = cudaLaunchAttributeClusterDimension;
+      at[0].val.clusterDim.x = n;
+      at[0].val.clusterDim.y = 1;
+      at[0].val.clusterDim.z = 1;
+      cfg.attrs = at;
+      cfg.numAttrs = 1;
+      e = cudaOccupancyMaxActiveClusters(&f.n[n], k_ragged<NT>, &cfg);
+    }
+    if (e != cudaSuccess || f.n[1] < 1) {
+      fail(W4A16_ECUDA, "linear: the device runs no CTA of the kernel (%s)", cudaGetErrorString(e));
+      return nullptr;
+    }
+    f.ready = true;
+  }
+  return f.n;
+}
+
+template <int NT>
 int launch_ragged(RaggedParams& p, const DeviceInfo* di, int max_units, bool weights_first, cudaStream_t st) {
-  const int fixed = sum_bytes<NT>() + 2 * kRMaxDepth * 8 + p.c.sets * 8 + (p.c.sets + 1) * 4;
+  const int fixed = fixed_bytes<NT>(p.c.sets);
   const int room = (di->smem_per_sm / 2 - di->smem_reserved - fixed) / stage_bytes<NT>();
   p.depth = room < kRMaxDepth ? room : kRMaxDepth;
   const int smem = fixed + p.depth * stage_bytes<NT>();
-  static std::atomic<bool> ready[64];
-  if (!ready[di->device & 63].load(std::memory_order_acquire)) {
-    W4_CUDA(cudaFuncSetAttribute(k_ragged<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, di->smem_optin));
-    ready[di->device & 63].store(true, std::memory_order_release);
-  }
-  const int slots = 2 * di->sms;
-  int S = slots / max_units;
-  S = S > 8 ? 8 : S;
-  S = S > p.c.G / 2 ? p.c.G / 2 : S;
-  p.splits = S < 1 ? 1 : S;
+  // Few units: as many CTAs share one as there are clusters for at once. (One more, and a last cluster starts when a first one ends:
+  // 5120 x 6144 at M = 1, 40 units: six 9.2 us, seven - of which 37 fit - 13.7; 5120 x 17408 17.6 and 24.0.)
+  const int* fit = clusters_at_once<NT>(di);
+  if (!fit) return W4A16_ECUDA;
+  const int slots = fit[1];
+  int S = 1;
+  for (int n = 2; n <= kRMaxSplit && n * kRGroups <= p.c.G; ++n)
+    if (max_units <= fit[n]) S = n;
+  p.splits = S;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute at[2];
   cfg.gridDim = dim3(p.splits > 1 ? p.splits * max_units : (max_units < slots ? max_units : slots));
