@@ -389,33 +389,34 @@ def linear_fused(y, w: Weights, x, M: int, s: Scratch, ln_weight=None, ln_eps: f
 ACT_NONE, ACT_SILU, ACT_GELU, ACT_GELU_TANH, ACT_SWIGLU = 0, 1, 2, 3, 4
 
 
-def _check_tensor(what: str, t, dtypes, rows: int, cols=None):
-    """`t` (None passes) must be contiguous, on the current device, of one of `dtypes` (names) and hold rows [x cols] elements."""
-    if t is None:
-        return
-    if str(t.dtype)[6:] not in dtypes:
-        raise W4A16Error(-1, f"{what}: {t.dtype}, not {' or '.join(dtypes)}")
-    if t.numel() != (rows if cols is None else rows * cols) or not t.is_contiguous():
-        raise W4A16Error(-1, f"{what}: {tuple(t.shape)}, not contiguous {rows if cols is None else (rows, cols)}")
-    if t.get_device() != _device():
-        raise W4A16Error(-1, f"{what}: on {t.device}, the current device is {_device()}")
+_BF16 = _F32 = _I32 = None
 
 
 def _device() -> int:
-    if _torch is None:
-        _stream()
+    """The current device; torch's types are looked up once on the way."""
+    global _torch, _BF16, _F32, _I32
+    if _BF16 is None:
+        import torch
+        _torch, _BF16, _F32, _I32 = torch, torch.bfloat16, torch.float32, torch.int32
     return _torch.cuda.current_device()
+
+
+def _want(what: str, t, kind, n: int, dev: int):
+    """`t` (None passes) must hold n contiguous elements of `kind` on device `dev`. (Some 0.3 us: small calls are bound by the host.)"""
+    if t is not None and (t.dtype is not kind or t.numel() != n or not t.is_contiguous() or t.get_device() != dev):
+        raise W4A16Error(-1, f"{what}: {tuple(t.shape)} {t.dtype} on {t.device}{'' if t.is_contiguous() else ', not contiguous'}; "
+                             f"wanted: {n} contiguous elements of {kind} on the current device, {dev}")
 
 
 def linear_epilogue(y, w: Weights, x, M: int, bias=None, activation: int = ACT_NONE, residual=None, stream=None):
     """y = act(x W^T + bias) + residual for any M; ACT_SWIGLU: w repacked by awq_repack_into_swiglu, y [M, out_f / 2], bias
     [gate | up]. residual may be y."""
-    cols = w.out_f // 2 if activation == ACT_SWIGLU else w.out_f
-    _check_tensor("linear_epilogue: x", x, ("bfloat16",), M, w.in_f)
-    _check_tensor("linear_epilogue: y", y, ("bfloat16",), M, cols)
-    _check_tensor("linear_epilogue: bias", bias, ("bfloat16",), w.out_f)
-    _check_tensor("linear_epilogue: residual", residual, ("bfloat16",), M, cols)
-    check(lib().w4a16_linear_epilogue(_ptr(y), C.byref(w), _ptr(x), M, _ptr(bias), activation, _ptr(residual), _stream(stream)))
+    dev, ny = _device(), M * w.out_f >> (1 if activation == ACT_SWIGLU else 0)
+    _want("linear_epilogue: x", x, _BF16, M * w.in_f, dev)
+    _want("linear_epilogue: y", y, _BF16, ny, dev)
+    _want("linear_epilogue: bias", bias, _BF16, w.out_f, dev)
+    _want("linear_epilogue: residual", residual, _BF16, ny, dev)
+    check(lib().w4a16_linear_epilogue(y.data_ptr(), C.byref(w), x.data_ptr(), M, _ptr(bias), activation, _ptr(residual), _stream(stream)))
 
 
 def experts_alloc(num_experts: int, out_f: int, in_f: int, group_size: int = 128) -> Experts:
@@ -439,13 +440,13 @@ def experts_linear(y, w: Experts, x, offsets, x_rows=None, bias=None, activation
     """y[p] = act(W_e x[x_rows[p]] + bias[e]) for the slots offsets[e] <= p < offsets[e + 1] of every expert e (x_rows None: x[p]).
     y [slots, out_f] (ACT_SWIGLU: out_f / 2 columns), x [tokens, in_f], offsets int32 [experts + 1], x_rows int32 [slots], as
     `route` gives them; rows of y behind the last slot stay as they were."""
-    slots = y.shape[0]
-    _check_tensor("experts_linear: y", y, ("bfloat16",), slots, w.out_f // 2 if activation == ACT_SWIGLU else w.out_f)
-    _check_tensor("experts_linear: x", x, ("bfloat16",), x.shape[0], w.in_f)
-    _check_tensor("experts_linear: offsets", offsets, ("int32",), w.num_experts + 1)
-    _check_tensor("experts_linear: x_rows", x_rows, ("int32",), slots)
-    _check_tensor("experts_linear: bias", bias, ("bfloat16",), w.num_experts, w.out_f)
-    check(lib().w4a16_experts_linear(_ptr(y), C.byref(w), _ptr(x), x.shape[0], _ptr(x_rows), _ptr(offsets), slots, _ptr(bias),
+    dev, slots, tokens, E = _device(), y.shape[0], x.shape[0], w.num_experts
+    _want("experts_linear: y", y, _BF16, slots * w.out_f >> (1 if activation == ACT_SWIGLU else 0), dev)
+    _want("experts_linear: x", x, _BF16, tokens * w.in_f, dev)
+    _want("experts_linear: offsets", offsets, _I32, E + 1, dev)
+    _want("experts_linear: x_rows", x_rows, _I32, slots, dev)
+    _want("experts_linear: bias", bias, _BF16, E * w.out_f, dev)
+    check(lib().w4a16_experts_linear(y.data_ptr(), C.byref(w), x.data_ptr(), tokens, _ptr(x_rows), offsets.data_ptr(), slots, _ptr(bias),
                                      activation, _stream(stream)))
 
 
@@ -464,6 +465,7 @@ class Route:
         self.offsets, self.rows = make(num_experts + 1), make(max_tokens * top_k)
         self.workspace_bytes = lib().w4a16_route_workspace(max_tokens, num_experts)
         self.workspace = make(self.workspace_bytes // 4)
+        self.pointers = [t.data_ptr() for t in (self.ids, self.weights, self.offsets, self.slots, self.rows)]
 
 
 def route_alloc(max_tokens: int, num_experts: int, top_k: int) -> Route:
@@ -476,23 +478,24 @@ def route(r: Route, logits, renormalize: bool = True, stream=None):
     T = logits.shape[0]
     if T > r.max_tokens:
         raise W4A16Error(-1, f"route: {T} tokens, room for {r.max_tokens}")
-    _check_tensor("route: logits", logits, ("float32", "bfloat16"), T, r.num_experts)
-    _check_tensor("route: workspace", r.workspace, ("int32",), r.workspace_bytes // 4)
-    check(lib().w4a16_route(_ptr(r.ids), _ptr(r.weights), _ptr(r.offsets), _ptr(r.slots), _ptr(r.rows), _ptr(logits),
-                            1 if logits.element_size() == 4 else 0, T, r.num_experts, r.top_k, 1 if renormalize else 0,
-                            _ptr(r.workspace), r.workspace_bytes, _stream(stream)))
+    dev, f32 = _device(), logits.dtype is _F32
+    _want("route: logits", logits, _F32 if f32 else _BF16, T * r.num_experts, dev)
+    _want("route: workspace", r.workspace, _I32, r.workspace_bytes // 4, dev)
+    check(lib().w4a16_route(*r.pointers, logits.data_ptr(), 1 if f32 else 0, T, r.num_experts, r.top_k, 1 if renormalize else 0,
+                            r.workspace.data_ptr(), r.workspace_bytes, _stream(stream)))
 
 
 def experts_combine(y, parts, slots, weights, residual=None, stream=None):
     """y[t] = residual[t] + sum over j of weights[t, j] * parts[slots[t, j]] (slots outside parts are empty). y, residual [T, hidden],
     parts [any, hidden], slots int32 and weights fp32 [T, top_k]; residual may be y."""
-    (T, hidden), top_k = y.shape, slots.shape[1]
-    _check_tensor("experts_combine: y", y, ("bfloat16",), T, hidden)
-    _check_tensor("experts_combine: parts", parts, ("bfloat16",), parts.shape[0], hidden)
-    _check_tensor("experts_combine: slots", slots, ("int32",), T, top_k)
-    _check_tensor("experts_combine: weights", weights, ("float32",), T, top_k)
-    _check_tensor("experts_combine: residual", residual, ("bfloat16",), T, hidden)
-    check(lib().w4a16_experts_combine(_ptr(y), _ptr(parts), parts.shape[0], _ptr(slots), _ptr(weights), _ptr(residual), T, top_k,
+    (T, hidden), k, dev = y.shape, slots.shape[1], _device()
+    rows = parts.shape[0]
+    _want("experts_combine: y", y, _BF16, T * hidden, dev)
+    _want("experts_combine: parts", parts, _BF16, rows * hidden, dev)
+    _want("experts_combine: slots", slots, _I32, T * k, dev)
+    _want("experts_combine: weights", weights, _F32, T * k, dev)
+    _want("experts_combine: residual", residual, _BF16, T * hidden, dev)
+    check(lib().w4a16_experts_combine(y.data_ptr(), parts.data_ptr(), rows, slots.data_ptr(), weights.data_ptr(), _ptr(residual), T, k,
                                       hidden, _stream(stream)))
 
 

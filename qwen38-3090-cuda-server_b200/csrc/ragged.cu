@@ -4,7 +4,7 @@
 // Mathematics: W = bf16((q - z) s), the value w4a16_dequant_rows gives, made in registers with packed bf16 arithmetic (every
 // step but the last exact) and multiplied by the bf16 activations on the tensor cores with fp32 sums, whatever the number of tokens.
 //
-// A unit of work is a 128-row tile of a set's weights with up to NT of its tokens (NT = 8, 16 or 32). A CTA takes a unit; where there are
+// A unit of work is a 128-row tile of a set's weights with up to NT of its tokens (NT = 8 or 16). A CTA takes a unit; where there are
 // few units, a cluster of S CTAs shares one, each a range of k groups, and adds up through distributed shared memory in a
 // fixed order (bitwise reproducible). In a CTA
 //   * one producer warp fills a ring of stages, a k group each: the 8576-byte weight block by one bulk copy (cp.async.bulk), each
@@ -45,53 +45,8 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Shared-memory loads at a 32-bit address plus a constant (the address arithmetic of generic pointers would double it)
-template <int OFF>
-__device__ __forceinline__ uint2 lds64(uint32_t a) {
-  uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2 + %3];" : "=r"(v.x), "=r"(v.y) : "r"(a), "n"(OFF));
-  return v;
-}
-template <int OFF>
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4 + %5];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a), "n"(OFF));
-  return v;
-}
-template <int OFF>
-__device__ __forceinline__ uint32_t lds_u16(uint32_t a) {
-  uint32_t v;
-  asm volatile("ld.shared.u16 %0, [%1 + %2];" : "=r"(v) : "r"(a), "n"(OFF));
-  return v;
-}
-template <int OFF>
-__device__ __forceinline__ uint32_t lds_u8(uint32_t a) {
-  uint32_t v;
-  asm volatile("ld.shared.u8 %0, [%1 + %2];" : "=r"(v) : "r"(a), "n"(OFF));
-  return v;
-}
-
-__device__ __forceinline__ uint32_t lds32(uint32_t a) {
-  uint32_t v;
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
-  return v;
-}
-__device__ __forceinline__ void sts32(uint32_t a, uint32_t v) { asm volatile("st.shared.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory"); }
 __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
-}
-
-// (a & mask) | bits in one instruction; written as such the compiler takes two, as it has room for one constant in each
-__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t bits) {
-  uint32_t d;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "r"(mask), "r"(bits));
-  return d;
-}
-
-__device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t d;
-  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-  return d;
 }
 
 // Where unit u of the launch lies: set, first slot, tokens, row tile. The chunks of one row tile are neighbours, so that its
@@ -172,10 +127,6 @@ __device__ __forceinline__ void multiply_group(float (&acc)[2][NT / 8][4], uint3
     tokens8(Const<0>());
     if constexpr (NT > 8)
       if (n > 8) tokens8(Const<1>());
-    if constexpr (NT > 16) {
-      if (n > 16) tokens8(Const<2>());
-      if (n > 24) tokens8(Const<3>());
-    }
   }
 }
 template <int NT, bool LARGE>
@@ -282,7 +233,7 @@ __global__ void __launch_bounds__(kRThreads, 2) k_ragged(const __grid_constant__
   if (warp == kRCons + 1) {
     // ================================================================ the rows' constants
     // Every lane of eight consumer lanes needs the same ones: made once, read by 16-byte loads. 34816 x 5120 at M = 1
-    // MEASURED.
+    // In place of eight small loads and eight permutes per lane and group: 1460 instructions per weight block instead of 1630 (M = 9).
     uint32_t ph = 0;
     for (int u = cluster; !dead && u < units; u += nclusters) {
       for (int g = g0; g < g1; g += kRGroups) {
@@ -457,7 +408,7 @@ const int* clusters_at_once(const DeviceInfo* di) {
 }
 
 template <int NT>
-int launch_ragged(RaggedParams& p, const DeviceInfo* di, int max_units, bool weights_first, cudaStream_t st) {
+int launch_ragged(RaggedParams& p, const DeviceInfo* di, int max_units, cudaStream_t st) {
   const int fixed = fixed_bytes<NT>(p.c.sets);
   const int room = (di->smem_per_sm / 2 - di->smem_reserved - fixed) / stage_bytes<NT>();
   p.depth = room < kRMaxDepth ? room : kRMaxDepth;
@@ -491,7 +442,6 @@ int launch_ragged(RaggedParams& p, const DeviceInfo* di, int max_units, bool wei
     at[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
     ++cfg.numAttrs;
   }
-  (void)weights_first;
   const cudaError_t err = cudaLaunchKernelEx(&cfg, k_ragged<NT>, p);
   return err == cudaSuccess ? W4A16_OK : fail(W4A16_ECUDA, "linear: launch: %s", cudaGetErrorString(err));
 }
@@ -519,20 +469,17 @@ int run_ragged(RaggedCall& c, const char* who, cudaStream_t st) {
   p.c = c;
   p.row_tiles = (c.N + kTileRows - 1) / kTileRows;
   p.status = di->status;
-  // Many tokens per set: whole tiles on tcgen05
-  if (c.sets == 1 && c.offsets == nullptr ? c.slots > 32 : c.slots > 32LL * c.sets) return launch_prefill_ragged(c, st);
+  // More than a few tokens per set: whole tiles on tcgen05, whose time hardly depends on their number up to 160 (here every eight
+  // tokens cost 64 mma.sync per weight block, beside 1040 instructions for its expansion). us, here / there: 16384 x 5120 at M = 8
+  // 15.5 / 17.1, at 16 19.0 / 17.3; 64 experts 2048 x 5120 with 4 slots each in the mean 89 / 107, with 8 111 / 107.
+  if (c.offsets ? c.slots > 6LL * c.sets : c.slots > 8) return launch_prefill_ragged(c, st);
   // chunks of NT tokens at most: every set with tokens has one more than its whole ones
   const int used = c.slots < c.sets ? c.slots : c.sets;
-  const int mean = (c.slots + c.sets - 1) / c.sets;
-  const int nt = mean <= 4 || (c.sets == 1 && c.slots <= 8) ? 8 : mean <= 10 || (c.sets == 1 && c.slots <= 16) ? 16 : 32;
-  const long long chunks = c.sets == 1 ? (c.slots + nt - 1) / nt : used + (c.slots - used) / nt;
-  const long long units = chunks * p.row_tiles;
+  const int nt = c.slots <= 4LL * c.sets || !c.offsets ? 8 : 16;
+  const long long units = static_cast<long long>(c.offsets ? used + (c.slots - used) / nt : 1) * p.row_tiles;
   W4_REQUIRE(units <= INT_MAX, "%s: %d slots x %d rows are too many for one call", who, c.slots, c.N);
   const int max_units = static_cast<int>(units);
-  const bool dense = c.offsets == nullptr;
-  if (nt == 8) return launch_ragged<8>(p, di, max_units, dense, st);
-  if (nt == 16) return launch_ragged<16>(p, di, max_units, dense, st);
-  return launch_ragged<32>(p, di, max_units, dense, st);
+  return nt == 8 ? launch_ragged<8>(p, di, max_units, st) : launch_ragged<16>(p, di, max_units, st);
 }
 
 int check_experts(const w4a16_experts_t* w) {

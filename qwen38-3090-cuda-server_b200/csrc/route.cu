@@ -1,5 +1,6 @@
 // Around the products grouped by expert: the router (softmax, top-k, slots sorted by expert) and the weighted combination of a token's
 // expert outputs.
+#include <atomic>
 #include <climits>
 #include <cfloat>
 
@@ -10,7 +11,7 @@ namespace {
 
 constexpr int kRouteWarps = 32;    // tokens of a block: one warp each, one bit each in the blocks' expert masks
 constexpr int kRouteMaxK = 16;
-constexpr int kCombineThreads = 128;
+constexpr int kCombineThreads = 128, kCombineCtas = 8;  // and CTAs per SM
 
 struct RouteParams {
   int32_t *ids, *offsets, *slots, *rows, *counts;
@@ -73,14 +74,24 @@ __global__ void __launch_bounds__(kRouteWarps * 32) k_route(const RouteParams p)
     }
     uint32_t my_key = 0, top = 0;
     float all = 0.f;  // sum of exp over every expert
-    for (int j = 0; j < p.k; ++j) {
-      uint32_t best = 0;
+    uint32_t best = 0;  // the lane's largest key and the first place that has it
+    int place = 0;
+    auto largest = [&]() {
+      best = key[0];
+      place = 0;
 #pragma unroll
-      for (int i = 0; i < EPL; ++i) best = max(best, key[i]);
-      best = __reduce_max_sync(0xffffffffu, best);
-      if (best == 0) break;  // nothing left to pick
+      for (int i = 1; i < EPL; ++i)
+        if (key[i] > best) {
+          best = key[i];
+          place = i;
+        }
+    };
+    largest();
+    for (int j = 0; j < p.k; ++j) {
+      const uint32_t most = __reduce_max_sync(0xffffffffu, best);
+      if (most == 0) break;  // nothing left to pick
       if (j == 0) {
-        top = best;
+        top = most;
         if (!p.renormalize) {
 #pragma unroll
           for (int i = 0; i < EPL; ++i)
@@ -89,17 +100,16 @@ __global__ void __launch_bounds__(kRouteWarps * 32) k_route(const RouteParams p)
           for (int d = 16; d; d /= 2) all += __shfl_xor_sync(0xffffffffu, all, d);
         }
       }
-      int at = INT_MAX;
+      const int at = __reduce_min_sync(0xffffffffu, best == most ? 32 * place + lane : INT_MAX);
+      if ((at & 31) == lane) {  // only this lane looks for its next largest
 #pragma unroll
-      for (int i = EPL - 1; i >= 0; --i)
-        if (key[i] == best) at = 32 * i + lane;
-      at = __reduce_min_sync(0xffffffffu, at);
-#pragma unroll
-      for (int i = 0; i < EPL; ++i)
-        if (32 * i + lane == at) key[i] = 0;
+        for (int i = 0; i < EPL; ++i)
+          if (i == place) key[i] = 0;
+        largest();
+      }
       if (lane == j) {
         my_id = at;
-        my_key = best;
+        my_key = most;
       }
     }
     float mine = my_id >= 0 ? expf(key_value(my_key) - key_value(top)) : 0.f;
@@ -134,25 +144,38 @@ __global__ void __launch_bounds__(kRouteWarps * 32) k_route(const RouteParams p)
   }
 }
 
-// counts[block][e] -> the number in earlier blocks, the totals go to row `blocks`. A warp per 32 experts walks the blocks.
-__global__ void __launch_bounds__(32) k_route_scan(const RouteParams p) {
+// counts[block][e] -> the number in earlier blocks; the totals go to row `blocks`. A CTA takes 32 experts, a warp a 32nd of the blocks:
+// sums of its part, a prefix sum over the warps, the part again.
+__global__ void __launch_bounds__(kRouteWarps * 32) k_route_scan(const RouteParams p) {
+  __shared__ int part[kRouteWarps][32];
   pdl_launch_dependents();
   pdl_wait();
-  const int e = blockIdx.x * 32 + threadIdx.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e = blockIdx.x * 32 + lane;
+  const int b0 = static_cast<int>(static_cast<long long>(p.blocks) * warp / kRouteWarps);
+  const int b1 = static_cast<int>(static_cast<long long>(p.blocks) * (warp + 1) / kRouteWarps);
+  int32_t* column = p.counts + e;
+  int sum = 0;
+  if (e < p.E)
+#pragma unroll 8
+    for (int b = b0; b < b1; ++b) sum += __ldcg(column + static_cast<size_t>(b) * p.E);
+  part[warp][lane] = sum;
+  __syncthreads();
   if (e >= p.E) return;
   int run = 0;
-  for (int b = 0; b < p.blocks; ++b) {
-    int32_t* at = p.counts + static_cast<size_t>(b) * p.E + e;
+  for (int w = 0; w < warp; ++w) run += part[w][lane];
+  for (int b = b0; b < b1; ++b) {
+    int32_t* at = column + static_cast<size_t>(b) * p.E;
     const int n = __ldcg(at);
     *at = run;
     run += n;
   }
-  p.counts[static_cast<size_t>(p.blocks) * p.E + e] = run;
+  if (warp == kRouteWarps - 1) column[static_cast<size_t>(p.blocks) * p.E] = run;
 }
 
+// Slots of a block's picks: first slot of the expert, picks of earlier blocks, earlier tokens of the block.
 __global__ void __launch_bounds__(kRouteWarps * 32) k_route_slots(const RouteParams p) {
   __shared__ uint32_t masks[kMaxSets];
-  __shared__ int offs[kMaxSets + 1];
+  __shared__ int offs[kMaxSets + 1], before[kMaxSets];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int t = blockIdx.x * kRouteWarps + warp;
   for (int e = tid; e < p.E; e += kRouteWarps * 32) masks[e] = 0;
@@ -161,16 +184,33 @@ __global__ void __launch_bounds__(kRouteWarps * 32) k_route_slots(const RoutePar
   pdl_wait();
   const int id = t < p.T && lane < p.k ? __ldcg(p.ids + static_cast<size_t>(t) * p.k + lane) : -1;
   if (id >= 0) atomicOr(&masks[id], 1u << warp);
-  for (int e = tid; e < p.E; e += kRouteWarps * 32) offs[e] = __ldcg(p.counts + static_cast<size_t>(p.blocks) * p.E + e);
+  for (int e = tid; e < p.E; e += kRouteWarps * 32) {
+    offs[e] = __ldcg(p.counts + static_cast<size_t>(p.blocks) * p.E + e);
+    before[e] = __ldcg(p.counts + static_cast<size_t>(blockIdx.x) * p.E + e);
+  }
   __syncthreads();
   if (warp == 0) scan_experts(offs, p.E, lane);
   __syncthreads();
   if (blockIdx.x == 0)
     for (int e = tid; e <= p.E; e += kRouteWarps * 32) p.offsets[e] = offs[e];
   if (id >= 0) {
-    const int slot = offs[id] + __ldcg(p.counts + static_cast<size_t>(blockIdx.x) * p.E + id) + __popc(masks[id] & ((1u << warp) - 1u));
+    const int slot = offs[id] + before[id] + __popc(masks[id] & ((1u << warp) - 1u));
     p.slots[static_cast<size_t>(t) * p.k + lane] = slot;
     p.rows[slot] = t;
+  }
+}
+
+// 16 bytes global -> shared by this thread, or zeros
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// All but the n latest groups of this thread have landed.
+__device__ __forceinline__ void cp_async_wait_but(int n) {
+  switch (n) {
+    case 2: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
+    case 4: asm volatile("cp.async.wait_group 4;" ::: "memory"); break;
+    default: asm volatile("cp.async.wait_group 7;" ::: "memory");
   }
 }
 
@@ -180,6 +220,8 @@ struct CombineParams {
   const int32_t* slots;
   const float* weights;
   int parts_rows, k, H;
+  uint32_t strips, items;  // strips of 256 columns, T x strips
+  int depth;               // 3, 5 or 8 items in the ring
 };
 
 __device__ __forceinline__ void add_row(float (&s)[8], const uint4& v, float w) {
@@ -191,46 +233,93 @@ __device__ __forceinline__ void add_row(float (&s)[8], const uint4& v, float w) 
   }
 }
 
-// A thread takes eight columns of a token; the loads of a token's rows are in flight together.
+// A warp takes 256 columns of a token at a time, eight per lane, its picks' rows by asynchronous copies through a ring of `depth` items in
+// shared memory: a lane copies and reads its own 16 bytes of every row only, so that no barrier is needed, and the bytes in
+// flight take no registers. Empty picks are filled with zeros. Bound by HBM: 4096 tokens of 8 picks x 5120, a tenth empty, 76 us (5.1 TB/s); with the
+// rows in registers (28 warps per SM, one item each) 100.
 __global__ void __launch_bounds__(kCombineThreads) k_combine(const CombineParams p) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t stage = p.k * 512 + kRouteMaxK * 4;  // rows, then the weights
+  const uint32_t ring = smem_u32(smem) + warp * p.depth * stage;
   pdl_launch_dependents();
   pdl_wait();
-  const int col = (blockIdx.y * kCombineThreads + threadIdx.x) * 8;
-  const size_t t = blockIdx.x;
-  if (col >= p.H) return;
-  float s[8] = {};
-  for (int j0 = 0; j0 < p.k; j0 += 8) {
-    uint4 v[8];
-    float w[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      w[j] = 0.f;
-      v[j] = make_uint4(0, 0, 0, 0);
-      if (j0 + j < p.k) {
-        const int slot = __ldcg(p.slots + t * p.k + j0 + j);
-        if (slot >= 0 && slot < p.parts_rows) {
-          w[j] = __ldcg(p.weights + t * p.k + j0 + j);
-          v[j] = __ldcg(reinterpret_cast<const uint4*>(p.parts + static_cast<size_t>(slot) * p.H + col));
-        }
-      }
+  const uint32_t stride = gridDim.x * (kCombineThreads / 32), first = blockIdx.x * (kCombineThreads / 32) + warp;
+  // lane j's pick j of an item, two steps before the item's copies start
+  auto pick = [&](uint32_t item, int& slot, float& w) {
+    slot = -1;
+    w = 0.f;
+    if (item < p.items && lane < p.k) {
+      const size_t o = static_cast<size_t>(item / p.strips) * p.k + lane;
+      slot = __ldcg(p.slots + o);
+      w = __ldcg(p.weights + o);
+      if (slot >= p.parts_rows) slot = -1;
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) add_row(s, v[j], w[j]);
+  };
+  auto start = [&](uint32_t item, uint32_t to, int slot, float w) {
+    if (item < p.items) {
+      const int col = static_cast<int>(item % p.strips) * 256 + lane * 8;
+      const bool inside = col < p.H;
+#pragma unroll 4
+      for (int j = 0; j < p.k; ++j) {
+        const int row = __shfl_sync(0xffffffffu, slot, j);
+        const bool real = row >= 0 && inside;
+        cp_async16(to + j * 512 + lane * 16, p.parts + (real ? static_cast<size_t>(row) * p.H + col : 0), real);
+      }
+      if (lane < p.k) sts32(to + p.k * 512 + lane * 4, __float_as_uint(slot >= 0 ? w : 0.f));
+    }
+    cp_async_commit();
+  };
+  int slot;
+  float weight;
+  pick(first, slot, weight);
+  uint32_t ahead = first;
+  for (int i = 0; i < p.depth - 1; ++i, ahead += stride) {
+    int next_slot;
+    float next_weight;
+    pick(ahead + stride, next_slot, next_weight);
+    start(ahead, ring + i * stage, slot, weight);
+    slot = next_slot;
+    weight = next_weight;
   }
-  const size_t o = t * p.H + col;
-  if (p.residual) add_row(s, *reinterpret_cast<const uint4*>(p.residual + o), 1.f);
-  uint32_t out[4];
+  int st = 0, st_ahead = p.depth - 1;
+  for (uint32_t item = first; item < p.items; item += stride, ahead += stride) {
+    int next_slot;
+    float next_weight;
+    pick(ahead + stride, next_slot, next_weight);
+    __syncwarp();  // every lane has read the weights that the stage held
+    start(ahead, ring + st_ahead * stage, slot, weight);
+    slot = next_slot;
+    weight = next_weight;
+    cp_async_wait_but(p.depth - 1);
+    __syncwarp();
+    const uint32_t t = item / p.strips, at = ring + st * stage;
+    const int col = static_cast<int>(item - t * p.strips) * 256 + lane * 8;
+    const size_t o = static_cast<size_t>(t) * p.H + col;
+    uint4 r = make_uint4(0, 0, 0, 0);
+    if (p.residual && col < p.H) r = *reinterpret_cast<const uint4*>(p.residual + o);
+    float s[8] = {};
+#pragma unroll 8
+    for (int j = 0; j < p.k; ++j) add_row(s, lds128<0>(at + j * 512 + lane * 16), __uint_as_float(lds32(at + p.k * 512 + j * 4)));
+    if (p.residual) add_row(s, r, 1.f);
+    if (col < p.H) {
+      uint32_t out[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) out[i] = float_to_bf16_bits(s[2 * i]) | (static_cast<uint32_t>(float_to_bf16_bits(s[2 * i + 1])) << 16);
-  *reinterpret_cast<uint4*>(p.y + o) = make_uint4(out[0], out[1], out[2], out[3]);
+      for (int i = 0; i < 4; ++i) out[i] = float_to_bf16_bits(s[2 * i]) | (static_cast<uint32_t>(float_to_bf16_bits(s[2 * i + 1])) << 16);
+      *reinterpret_cast<uint4*>(p.y + o) = make_uint4(out[0], out[1], out[2], out[3]);
+    }
+    if (++st == p.depth) st = 0;
+    if (++st_ahead == p.depth) st_ahead = 0;
+  }
 }
 
 template <class Kernel, class Params>
-int enqueue(Kernel kernel, dim3 grid, int threads, const Params& p, void* stream, const char* who) {
+int enqueue(Kernel kernel, dim3 grid, int threads, const Params& p, void* stream, const char* who, int smem = 0) {
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute at[1];
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = static_cast<cudaStream_t>(stream);
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
@@ -289,7 +378,7 @@ int w4a16_route(int32_t* ids, float* weights, int32_t* offsets, int32_t* slots, 
   else if (per_lane <= 8) rc = enqueue(k_route<8>, grid, kRouteWarps * 32, p, stream, "route");
   else rc = enqueue(k_route<16>, grid, kRouteWarps * 32, p, stream, "route");
   if (rc != W4A16_OK || blocks <= 1) return rc;
-  rc = enqueue(k_route_scan, dim3((num_experts + 31) / 32), 32, p, stream, "route");
+  rc = enqueue(k_route_scan, dim3((num_experts + 31) / 32), kRouteWarps * 32, p, stream, "route");
   if (rc != W4A16_OK) return rc;
   return enqueue(k_route_slots, grid, kRouteWarps * 32, p, stream, "route");
 }
@@ -298,7 +387,7 @@ int w4a16_experts_combine(uint16_t* y, const uint16_t* parts, int parts_rows, co
                           const uint16_t* residual, int T, int top_k, int hidden, void* stream) {
   W4_REQUIRE(T >= 0 && parts_rows >= 0, "experts_combine: %d tokens, %d rows", T, parts_rows);
   W4_REQUIRE(top_k >= 1 && top_k <= kRouteMaxK, "experts_combine: top_k %d (1..%d)", top_k, kRouteMaxK);
-  W4_REQUIRE(hidden > 0 && hidden % 8 == 0 && hidden <= 8 * kCombineThreads * 65535, "experts_combine: hidden %d not a positive multiple of 8", hidden);
+  W4_REQUIRE(hidden > 0 && hidden % 8 == 0, "experts_combine: hidden %d not a positive multiple of 8", hidden);
   if (T == 0) return W4A16_OK;
   W4_REQUIRE(y != nullptr && slots != nullptr && weights != nullptr && (parts != nullptr || parts_rows == 0), "experts_combine: null argument");
   W4_REQUIRE(((reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(parts) | reinterpret_cast<uintptr_t>(residual)) & 15) == 0,
@@ -307,9 +396,23 @@ int w4a16_experts_combine(uint16_t* y, const uint16_t* parts, int parts_rows, co
   const size_t yb = static_cast<size_t>(T) * hidden * 2;
   W4_REQUIRE(ranges_apart(parts, static_cast<size_t>(parts_rows) * hidden * 2, y, yb), "experts_combine: y overlaps parts");
   W4_REQUIRE(residual == nullptr || residual == y || ranges_apart(residual, yb, y, yb), "experts_combine: residual overlaps y but is not y");
-  const CombineParams p = {y, parts, residual, slots, weights, parts_rows, top_k, hidden};
-  const dim3 grid(T, (hidden / 8 + kCombineThreads - 1) / kCombineThreads);
-  return enqueue(k_combine, grid, kCombineThreads, p, stream, "experts_combine");
+  const DeviceInfo* di = device_info();
+  if (!di) return W4A16_ECUDA;
+  const uint32_t strips = (static_cast<uint32_t>(hidden) + 255) / 256;
+  W4_REQUIRE(static_cast<unsigned long long>(T) * strips <= INT_MAX, "experts_combine: %d tokens x %d are too many for one call", T, hidden);
+  // some 24 rows of 512 bytes in flight per warp, four CTAs of four warps per SM
+  const int depth = top_k <= 3 ? 8 : top_k <= 5 ? 5 : 3;
+  const CombineParams p = {y, parts, residual, slots, weights, parts_rows, top_k, hidden, strips, static_cast<uint32_t>(T) * strips, depth};
+  const int smem = kCombineThreads / 32 * depth * (top_k * 512 + kRouteMaxK * 4);
+  static std::atomic<bool> ready[64];
+  if (!ready[di->device & 63].load(std::memory_order_acquire)) {
+    W4_CUDA(cudaFuncSetAttribute(k_combine, cudaFuncAttributeMaxDynamicSharedMemorySize, di->smem_optin));
+    ready[di->device & 63].store(true, std::memory_order_release);
+  }
+  const int fit = di->smem_per_sm / (smem + di->smem_reserved);
+  const uint32_t ctas = (p.items + kCombineThreads / 32 - 1) / (kCombineThreads / 32);
+  const uint32_t most = static_cast<uint32_t>(di->sms) * (fit < kCombineCtas ? fit : kCombineCtas);
+  return enqueue(k_combine, dim3(ctas < most ? ctas : most), kCombineThreads, p, stream, "experts_combine", smem);
 }
 
 }  // extern "C"
