@@ -53,7 +53,6 @@ constexpr int EW = 8;                       // epilogue warps: two per lane quar
 constexpr int kWEpi0 = PW, kWWeights = PW + EW, kWIssue = kWWeights + 1, kWActs = kWIssue + 1;
 constexpr int kPWarps = kWActs + 1;
 constexpr int kPGather = 3;                 // with sets: warps that gather rows, kWActs and the ones behind it
-constexpr int kPRows = 2 * kTileRows;       // output rows of a CTA pair's tile
 constexpr int kPMaxTN = 256;                // tokens of a tile: a multiple of 32 (the pair's MMA needs N % 32 == 0)
 constexpr int kPMaxSplit = 4;               // 2 S <= 8 CTAs: the portable cluster size
 constexpr int kPSteps = 4;                  // activation stages, each one k group of the CTA's TN / 2 tokens
@@ -68,6 +67,8 @@ constexpr int kPBars = 2 * kPMaxWD + kPDone + kPMaxA + kPSteps + 2;
 // Tensor memory: the accumulator's TN columns, the rest are slots of the A operand, 64 columns per k group.
 __host__ __device__ constexpr int a_slots(int tn) { return tn <= 128 ? 6 : 4; }
 constexpr int kPSetsTN = 160;               // tokens of a tile with sets
+constexpr int kPSingleTN = 80, kPSingleMean = 48;  // tokens of a tile of a CTA alone at most; mean set up to which sets take such
+static_assert(kPSingleTN <= kPSetsTN / 2, "lists of rows");
 static_assert(128 + 6 * 64 <= 512 && 256 + 4 * 64 <= 512 && kPMaxA <= kPDone && kPSteps <= kPDone, "ring depths");
 
 struct PrefillParams {
@@ -102,6 +103,13 @@ __host__ __device__ constexpr int prefill_warps(int mode) { return mode == kSets
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+template <bool PAIR>  // the pair leader's barrier (a mapped address), or this CTA's own
+__device__ __forceinline__ void arrive_at(uint32_t bar) {
+  if constexpr (PAIR)
+    mbar_arrive_cluster(bar);
+  else
+    mbar_arrive(bar);
+}
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t smem_dst, uint32_t ncols) {
   asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_dst), "r"(ncols) : "memory");
   asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
@@ -115,6 +123,14 @@ __device__ __forceinline__ void umma_bf16_ts_pair(uint32_t d_tmem, uint32_t a_tm
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// The same for a CTA alone: 128 rows, all of the columns from its own shared memory
+__device__ __forceinline__ void umma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
       "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
@@ -133,13 +149,27 @@ __device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* m
       "l"(map), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
-// Four rows of 64 k, each of its own, into 512 consecutive bytes (with the swizzle of their place in a 1024-byte atom).
-__device__ __forceinline__ void tma_gather_pair(uint32_t dst, const CUtensorMap* map, int x, const int4& rows, uint32_t bar) {
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
   asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2 "
-      "[%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
-      "l"(map), "r"(x), "r"(rows.x), "r"(rows.y), "r"(rows.z), "r"(rows.w), "r"(bar)
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(bar)
       : "memory");
+}
+// Four rows of 64 k, each of its own, into 512 consecutive bytes (with the swizzle of their place in a 1024-byte atom).
+template <bool PAIR>
+__device__ __forceinline__ void tma_gather(uint32_t dst, const CUtensorMap* map, int x, const int4& rows, uint32_t bar) {
+  if constexpr (PAIR)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2 "
+        "[%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(rows.x), "r"(rows.y), "r"(rows.z), "r"(rows.w), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(rows.x), "r"(rows.y), "r"(rows.z), "r"(rows.w), "r"(bar)
+        : "memory");
 }
 // K-major operand descriptor for a 128-byte-swizzled tile ([row][128 B], 8-row groups 1024 B apart)
 __device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t saddr) {
@@ -152,6 +182,12 @@ __device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t saddr) {
 struct PTile {
   int pair, tok0, n, toks, set;
 };
+// tokens are multiplied in steps of 32 by a pair, of 16 by a CTA alone
+template <bool PAIR>
+__device__ __forceinline__ int mma_tokens(int n) {
+  return PAIR ? (n + 31) & ~31 : (n + 15) & ~15;
+}
+template <bool PAIR>
 __device__ __forceinline__ PTile tile_of(const PrefillParams& p, int tile) {
   const int nfull = p.pairs * p.full_tt;
   PTile t;
@@ -162,7 +198,7 @@ __device__ __forceinline__ PTile tile_of(const PrefillParams& p, int tile) {
   } else {
     t.pair = tile - nfull;
     t.tok0 = p.full_tt * p.tn;
-    t.n = (p.M - t.tok0 + 31) & ~31;
+    t.n = mma_tokens<PAIR>(p.M - t.tok0);
   }
   t.toks = min(t.n, p.M - t.tok0);
   t.set = 0;
@@ -176,12 +212,12 @@ struct SetTable {
   const int* first;  // [sets + 1]
 };
 // A role's walk over the tiles of its cluster; `set` moves on only.
-template <int MODE>
+template <int MODE, bool PAIR>
 __device__ __forceinline__ PTile walk_tile(const PrefillParams& p, int tile, int& set, const SetTable& tab) {
-  if constexpr (MODE != kSets) return tile_of(p, tile);
+  if constexpr (MODE != kSets) return tile_of<PAIR>(p, tile);
   while (set + 1 < p.call.sets && tile >= tab.first[set + 1]) ++set;
   const int2 b = tab.bounds[set];
-  const int n = b.y - b.x, tt = (n + p.tn - 1) / p.tn, per = ((n + tt - 1) / tt + 31) & ~31;
+  const int n = b.y - b.x, tt = (n + p.tn - 1) / p.tn, per = mma_tokens<PAIR>((n + tt - 1) / tt);
   const int at = tile - tab.first[set];
   PTile t;
   t.set = set;
@@ -189,7 +225,7 @@ __device__ __forceinline__ PTile walk_tile(const PrefillParams& p, int tile, int
   const int c = (at - t.pair * tt) * per;
   t.tok0 = b.x + c;
   t.toks = min(per, n - c);
-  t.n = (t.toks + 31) & ~31;
+  t.n = mma_tokens<PAIR>(t.toks);
   return t;
 }
 
@@ -263,11 +299,13 @@ __device__ __forceinline__ void finish_four(const RaggedCall& c, int N, int tok,
     }
 }
 
-template <int MODE>
+template <int MODE, bool PAIR>
 __global__ void __launch_bounds__(prefill_warps(MODE) * 32, 1) k_prefill(const __grid_constant__ PrefillParams p) {
+  constexpr int CG = PAIR ? 2 : 1;  // CTAs of a tile
+
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const int xbytes = p.tn * 128;  // one activation stage: two swizzled tiles of TN / 2 tokens x 64 k
+  const int xbytes = p.tn / CG * 256;  // one activation stage: two swizzled tiles of this CTA's share of TN tokens x 64 k
   uint8_t* xbuf = smem;          // 128-byte-swizzled TMA tiles start on 1024-byte boundaries
   uint8_t* cbuf = xbuf + kPSteps * xbytes;  // [TN tokens][128 rows] bf16: the finished tile on its way out
   uint8_t* ring = cbuf + p.tn * (kTileRows * 2);
@@ -276,8 +314,8 @@ __global__ void __launch_bounds__(prefill_warps(MODE) * 32, 1) k_prefill(const _
 
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-  const uint32_t rank = cluster_rank(), leader = rank & ~1u;
-  const int half = static_cast<int>(rank & 1u), split = static_cast<int>(rank >> 1);
+  const uint32_t rank = cluster_rank(), leader = PAIR ? rank & ~1u : rank;
+  const int half = PAIR ? static_cast<int>(rank & 1u) : 0, split = static_cast<int>(PAIR ? rank >> 1 : rank);
   const int WD = p.wdepth, S = p.splits;
   const int na = a_slots(p.tn);
   const uint32_t ring_a = smem_u32(ring), xbuf_a = smem_u32(xbuf);
@@ -297,12 +335,17 @@ __global__ void __launch_bounds__(prefill_warps(MODE) * 32, 1) k_prefill(const _
     for (int i = 0; i < kPDone; ++i) mbar_init(done_a + i * 8, 1);
     // activations: one arrival that expects both CTAs' bytes; gathered rows: one arrival of each CTA
     for (int i = 0; i < kPSteps; ++i) mbar_init(xfull_a + i * 8, 1);
-    for (int i = 0; i < kPMaxA; ++i) mbar_init(afull_a + i * 8, 8);
+    for (int i = 0; i < kPMaxA; ++i) mbar_init(afull_a + i * 8, 4 * CG);
     mbar_init(dfull_a, 1);
-    mbar_init(dempty_a, 2 * EW);
+    mbar_init(dempty_a, CG * EW);
     fence_mbar_init();
   }
-  if (warp == kWIssue) tmem_alloc_pair(smem_u32(tmem_slot), kPTmemCols);
+  if (warp == kWIssue) {
+    if constexpr (PAIR)
+      tmem_alloc_pair(smem_u32(tmem_slot), kPTmemCols);
+    else
+      tmem_alloc(smem_u32(tmem_slot), kPTmemCols);
+  }
   tc_fence_before();
   __syncthreads();
   cluster_sync();  // the other CTAs' barriers exist from here on
@@ -343,7 +386,7 @@ __global__ void __launch_bounds__(prefill_warps(MODE) * 32, 1) k_prefill(const _
     __syncthreads();
     tiles = first[p.call.sets];
   }
-  const int cluster = blockIdx.x / (2 * S), nclusters = gridDim.x / (2 * S);
+  const int cluster = blockIdx.x / (CG * S), nclusters = gridDim.x / (CG * S);
   const int g0 = p.G * split / S, g1 = p.G * (split + 1) / S;  // this split's k groups (S <= G)
   bool dead = false;
 
@@ -353,8 +396,8 @@ __global__ void __launch_bounds__(prefill_warps(MODE) * 32, 1) k_prefill(const _
       int st = 0;
       uint32_t ph = 1;
       for (int tile = cluster; !dead && tile < tiles; tile += nclusters) {
-        const PTile t = walk_tile<MODE>(p, tile, set, tab);
-        const int rt = min(2 * t.pair + half, p.row_tiles - 1);
+        const PTile t = walk_tile<MODE, PAIR>(p, tile, set, tab);
+        const int rt = min(CG * t.pair + half, p.row_tiles - 1);
         const uint8_t* src = p.stream + (static_cast<size_t>(rt) * p.G + g0) * kTileGroupBytes;
         if constexpr (MODE == kSets) src += p.call.set_bytes * t.set;
         for (int g = g0; g < g1; ++g, src += kTileGroupBytes) {
@@ -379,13 +422,13 @@ __global__ void __launch_bounds__(prefill_warps(MODE) * 32, 1) k_prefill(const _
     // ================================================================ MMA issuer (leader CTA only)
     // The whole warp walks (so that the operands stay in uniform registers), one elected lane issues.
     if (half == 0) {
-      const uint16_t both = static_cast<uint16_t>(3u << rank);
+      const uint16_t both = static_cast<uint16_t>(3u << rank);  // (a pair's two CTAs)
       const uint64_t desc0 = umma_desc_sw128(xbuf_a);
       const uint32_t x16 = static_cast<uint32_t>(xbytes) >> 4;
       uint32_t j = 0, aph = 0, dph = 1;
       int a = 0;
       for (int tile = cluster; !dead && tile < tiles; tile += nclusters, dph ^= 1) {
-        const uint32_t idesc = umma_idesc_bf16(kPRows, walk_tile<MODE>(p, tile, set, tab).n);
+        const uint32_t idesc = umma_idesc_bf16(CG * kTileRows, walk_tile<MODE, PAIR>(p, tile, set, tab).n);
         if (!warp_agrees(mbar_wait_bounded(dempty_a, dph, kPSpin))) dead = true;  // (passes on the first tile)
         for (int g = g0; !dead && g < g1; ++g, ++j) {
           const uint32_t st = j & (kPSteps - 1);
@@ -400,10 +443,19 @@ __global__ void __launch_bounds__(prefill_warps(MODE) * 32, 1) k_prefill(const _
           const uint32_t at = tmem_a + a * 64;
           if (elect_one()) {
 #pragma unroll
-            for (int s = 0; s < 8; ++s)
-              umma_bf16_ts_pair(tmem, at + s * 8, (s < 4 ? b0 : b1) + 2 * (s & 3), idesc, s > 0 || g > g0);
-            umma_commit_pair(done_a + (j & (kPDone - 1)) * 8, both);
-            if (g == g1 - 1) umma_commit_pair(dfull_a, both);
+            for (int s = 0; s < 8; ++s) {
+              if constexpr (PAIR)
+                umma_bf16_ts_pair(tmem, at + s * 8, (s < 4 ? b0 : b1) + 2 * (s & 3), idesc, s > 0 || g > g0);
+              else
+                umma_bf16_ts(tmem, at + s * 8, (s < 4 ? b0 : b1) + 2 * (s & 3), idesc, s > 0 || g > g0);
+            }
+            if constexpr (PAIR) {
+              umma_commit_pair(done_a + (j & (kPDone - 1)) * 8, both);
+              if (g == g1 - 1) umma_commit_pair(dfull_a, both);
+            } else {
+              umma_commit(done_a + (j & (kPDone - 1)) * 8);
+              if (g == g1 - 1) umma_commit(dfull_a);
+            }
           }
           __syncwarp();
           if (++a == na) {
@@ -423,18 +475,18 @@ __global__ void __launch_bounds__(prefill_warps(MODE) * 32, 1) k_prefill(const _
       // the last one. Issuing a load takes a warp some 25 cycles and a group has up to 40, so three warps take the groups in turn, each with
       // its own list of rows. 64 experts 2048 x 5120 of 8 picks, us at 300 / 1200 / 4096 tokens: one warp (a shuffle per row) 232 / 460 /
       // 1270, two 178 / 319 / 831, with lists 145 / 267 / 675, three 140 / 245 / 623, four the same; rows already in slot order 133 / 216 / 548.
-      const uint32_t xfull_l = map_to_rank(xfull_a, leader);
+      const uint32_t xfull_l = PAIR ? map_to_rank(xfull_a, leader) : xfull_a;
       int* rows = reinterpret_cast<int*>(bars + kPBars + 2) + (warp - kWActs) * (kPSetsTN / 2);  // (16-byte aligned)
       uint32_t j = 0;
       for (int tile = cluster; !dead && tile < tiles; tile += nclusters) {
-        const PTile t = walk_tile<MODE>(p, tile, set, tab);
+        const PTile t = walk_tile<MODE, PAIR>(p, tile, set, tab);
         __syncwarp();
-        for (int i = lane; i < t.n >> 1; i += 32) {
-          const int slot = t.tok0 + min(half * (t.n >> 1) + i, t.toks - 1);
+        for (int i = lane; i < t.n / CG; i += 32) {
+          const int slot = t.tok0 + min(half * (t.n / CG) + i, t.toks - 1);
           rows[i] = min(max(__ldcg(p.call.x_rows + slot), 0), p.call.x_tokens - 1);  // (no read outside x, whatever the rows hold)
         }
         __syncwarp();
-        const int fours = t.n / 8;
+        const int fours = t.n / (4 * CG);
         for (int g = g0; g < g1; ++g, ++j) {
           if (j % kPGather != static_cast<uint32_t>(warp - kWActs)) continue;
           const uint32_t st = j & (kPSteps - 1);
@@ -450,8 +502,8 @@ __global__ void __launch_bounds__(prefill_warps(MODE) * 32, 1) k_prefill(const _
 #pragma unroll 4
             for (int i = 0; i < fours; ++i) {
               const int4 rr = *reinterpret_cast<const int4*>(rows + 4 * i);
-              tma_gather_pair(dst + i * 512, &p.amap, g * kGroup, rr, xfull_l + st * 8);
-              tma_gather_pair(dst + i * 512 + (xbytes >> 1), &p.amap, g * kGroup + 64, rr, xfull_l + st * 8);
+              tma_gather<PAIR>(dst + i * 512, &p.amap, g * kGroup, rr, xfull_l + st * 8);
+              tma_gather<PAIR>(dst + i * 512 + (xbytes >> 1), &p.amap, g * kGroup + 64, rr, xfull_l + st * 8);
             }
           }
           __syncwarp();
@@ -464,12 +516,12 @@ __global__ void __launch_bounds__(prefill_warps(MODE) * 32, 1) k_prefill(const _
       }
       __syncwarp();
     } else if (warp == kWActs && lane == 0) {
-      const uint32_t xfull_l = map_to_rank(xfull_a, leader);
+      const uint32_t xfull_l = PAIR ? map_to_rank(xfull_a, leader) : xfull_a;
       pdl_wait();  // the previous kernel produced the activations (the weights never depend on it)
       uint32_t j = 0;
       for (int tile = cluster; !dead && tile < tiles; tile += nclusters) {
-        const PTile t = walk_tile<MODE>(p, tile, set, tab);
-        const int y = t.tok0 + half * (t.n >> 1);
+        const PTile t = walk_tile<MODE, PAIR>(p, tile, set, tab);
+        const int y = t.tok0 + half * (t.n / CG);
         for (int g = g0; g < g1; ++g, ++j) {
           const uint32_t st = j & (kPSteps - 1);
           const uint32_t jd = j - kPSteps;
@@ -478,9 +530,14 @@ __global__ void __launch_bounds__(prefill_warps(MODE) * 32, 1) k_prefill(const _
             dead = true;
             break;
           }
-          if (half == 0) mbar_expect_tx(xfull_a + st * 8, 2 * xbytes);
-          tma_load_pair(xbuf_a + st * xbytes, &p.amap, g * kGroup, y, xfull_l + st * 8);
-          tma_load_pair(xbuf_a + st * xbytes + (xbytes >> 1), &p.amap, g * kGroup + 64, y, xfull_l + st * 8);
+          if (half == 0) mbar_expect_tx(xfull_a + st * 8, CG * xbytes);
+          if constexpr (PAIR) {
+            tma_load_pair(xbuf_a + st * xbytes, &p.amap, g * kGroup, y, xfull_l + st * 8);
+            tma_load_pair(xbuf_a + st * xbytes + (xbytes >> 1), &p.amap, g * kGroup + 64, y, xfull_l + st * 8);
+          } else {
+            tma_load(xbuf_a + st * xbytes, &p.amap, g * kGroup, y, xfull_l + st * 8);
+            tma_load(xbuf_a + st * xbytes + (xbytes >> 1), &p.amap, g * kGroup + 64, y, xfull_l + st * 8);
+          }
         }
       }
       if (dead && half == 0) {
@@ -500,7 +557,7 @@ __global__ void __launch_bounds__(prefill_warps(MODE) * 32, 1) k_prefill(const _
     const int q = warp & 3, team = warp >> 2;
     const int row = q * 32 + lane;
     const uint32_t a_t = tmem_a + (static_cast<uint32_t>(q * 32) << 16);
-    const uint32_t afull_l = map_to_rank(afull_a, leader);
+    const uint32_t afull_l = PAIR ? map_to_rank(afull_a, leader) : afull_a;
     const int ntiles = cluster < tiles ? (tiles - 1 - cluster) / nclusters + 1 : 0;
     const uint32_t ngroups = static_cast<uint32_t>(ntiles) * static_cast<uint32_t>(g1 - g0);
     const uint32_t off_e = weight_slot(row, 0) * 16, off_o = kChunkBytes + weight_slot(row, 1) * 16;  // even and odd 32-k chunks
@@ -578,7 +635,7 @@ __global__ void __launch_bounds__(prefill_warps(MODE) * 32, 1) k_prefill(const _
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(afull_l + a * 8);
+      if (lane == 0) arrive_at<PAIR>(afull_l + a * 8);
       if ((a += kPTeams) >= na) a -= na;
       if ((st += kPTeams) >= WD) {
         st -= WD;
@@ -592,7 +649,7 @@ __global__ void __launch_bounds__(prefill_warps(MODE) * 32, 1) k_prefill(const _
     // the stores to C, 256 bytes per token, run beside the next tile's main loop.
     const int q = warp & 3, eh = (warp - kWEpi0) >> 2, et = tid - kWEpi0 * 32;
     const uint32_t lane_t = tmem + (static_cast<uint32_t>(q * 32) << 16);
-    const uint32_t dempty_l = map_to_rank(dempty_a, leader);
+    const uint32_t dempty_l = PAIR ? map_to_rank(dempty_a, leader) : dempty_a;
     uint32_t dph = 0;
     // Layers with an epilogue: the sums are finished in registers on their way out, in fp32. The residual's tile waits in the
     // staging buffer by then, brought in beside the main loop.
@@ -600,7 +657,7 @@ __global__ void __launch_bounds__(prefill_warps(MODE) * 32, 1) k_prefill(const _
       const RaggedCall& c = p.call;
       const bool gated = c.act == W4A16_ACT_SWIGLU;
       const int w8 = gated ? 3 : 4;                              // log2 of the eights of columns per token
-      const int r0 = (2 * t.pair + half) * kTileRows;
+      const int r0 = (CG * t.pair + half) * kTileRows;
       const int cols = min(kTileRows, p.N - r0) >> (gated ? 1 : 0);  // (<= 0: an odd last row tile's second half)
       const int col0 = gated ? r0 >> 1 : r0, cl = (et & ((1 << w8) - 1)) * 8;
       uint16_t* cs = reinterpret_cast<uint16_t*>(cbuf);
@@ -630,7 +687,7 @@ __global__ void __launch_bounds__(prefill_warps(MODE) * 32, 1) k_prefill(const _
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(dempty_l);
+        if (lane == 0) arrive_at<PAIR>(dempty_l);
       }
       named_bar_sync(1, EW * 32);  // every epilogue warp comes here for every tile, dead or not
       if (cl < cols && !dead)
@@ -640,7 +697,7 @@ __global__ void __launch_bounds__(prefill_warps(MODE) * 32, 1) k_prefill(const _
     };
     if constexpr (MODE != kPlain) pdl_wait();  // bias and residual may come from the kernel in front
     for (int tile = cluster; tile < tiles; tile += nclusters, dph ^= 1) {
-      const PTile t = walk_tile<MODE>(p, tile, set, tab);
+      const PTile t = walk_tile<MODE, PAIR>(p, tile, set, tab);
       uint16_t* cs = reinterpret_cast<uint16_t*>(cbuf);
       if constexpr (MODE != kPlain) {
         finish_tile(t, dph);
@@ -662,10 +719,10 @@ __global__ void __launch_bounds__(prefill_warps(MODE) * 32, 1) k_prefill(const _
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(dempty_l);
+        if (lane == 0) arrive_at<PAIR>(dempty_l);
       }
       named_bar_sync(1, EW * 32);  // every epilogue warp comes here for every tile, dead or not
-      const int r0 = (2 * t.pair + half) * kTileRows;
+      const int r0 = (CG * t.pair + half) * kTileRows;
       const int rows = min(kTileRows, p.N - r0);                     // (<= 0: an odd last row tile's second half)
       const int toks = dead ? 0 : min(t.n, p.M - t.tok0);
       if (p.wide) {
@@ -697,7 +754,7 @@ __global__ void __launch_bounds__(prefill_warps(MODE) * 32, 1) k_prefill(const _
     // Every split's fp32 tile goes to its own shared memory (the activation stages: all MMAs have read them, and
     // [TN tokens][128 rows] floats are exactly their size), then split s adds up and stores the s-th share
     // of the tokens, reading the others' tiles through the cluster.
-    const PTile t = tile_of(p, cluster);
+    const PTile t = tile_of<PAIR>(p, cluster);
     if (warp >= kWEpi0 && warp < kWEpi0 + EW) {
       const int q = warp & 3;
       const uint32_t lane_t = tmem + (static_cast<uint32_t>(q * 32) << 16);
@@ -724,11 +781,11 @@ __global__ void __launch_bounds__(prefill_warps(MODE) * 32, 1) k_prefill(const _
       // thread, 4-byte loads and 64-byte runs of C took 1.6 us of a 5120 x 6144 launch at M = 77. The four layers of a block at M = 77,
       // three of which split: 85.1 -> 83.8 us, at M = 40 80.7 -> 79.9.)
       const int c0 = t.n * split / S, n4 = (t.n * (split + 1) / S - c0) * (kTileRows / 4);
-      const int r0 = (2 * t.pair + half) * kTileRows;
+      const int r0 = (CG * t.pair + half) * kTileRows;
       uint32_t src[kPMaxSplit];
 #pragma unroll
       for (int s = 0; s < kPMaxSplit; ++s)
-        src[s] = map_to_rank(xbuf_a, static_cast<uint32_t>(2 * min(s, S - 1) + half)) + c0 * (kTileRows * 4);
+        src[s] = map_to_rank(xbuf_a, static_cast<uint32_t>(CG * min(s, S - 1) + half)) + c0 * (kTileRows * 4);
 #pragma unroll 2
       for (int i = tid; i < n4; i += (PW + EW) * 32) {
         const int r = r0 + 4 * (i & (kTileRows / 4 - 1)), tok = t.tok0 + c0 + i / (kTileRows / 4);
@@ -776,7 +833,10 @@ __global__ void __launch_bounds__(prefill_warps(MODE) * 32, 1) k_prefill(const _
   cluster_sync();
   if (warp == kWIssue) {
     tc_fence_after();
-    tmem_dealloc_pair(tmem, kPTmemCols);
+    if constexpr (PAIR)
+      tmem_dealloc_pair(tmem, kPTmemCols);
+    else
+      tmem_dealloc(tmem, kPTmemCols);
   }
   // every store of this CTA was issued before the barrier above: its share of the launch's completion signal
   if (p.comm_local && tid == 0) signal_cta_done(p.comm_local, p.comm_peers, p.comm_n, p.comm_rank);
@@ -784,11 +844,12 @@ __global__ void __launch_bounds__(prefill_warps(MODE) * 32, 1) k_prefill(const _
 
 // ------------------------------------------------------------------ the plan of a launch
 struct PrefillPlan {
+  bool pair = true;
   int tn = 0, splits = 1, full_tt = 0, tiles = 0, clusters = 0, wdepth = 0, smem = 0;
 };
 
-int prefill_smem(int tn, int wdepth) {
-  return 1024 + kPSteps * tn * 128 + tn * kTileRows * 2 + wdepth * kTileGroupBytes + kPBars * 8 + 16;
+int prefill_smem(bool pair, int tn, int wdepth) {
+  return 1024 + kPSteps * tn * (pair ? 128 : 256) + tn * kTileRows * 2 + wdepth * kTileGroupBytes + kPBars * 8 + 16;
 }
 
 // Tokens per tile and K splits. A cluster's time for a tile is its k groups times the slower of the tensor cores
@@ -840,9 +901,27 @@ PrefillPlan plan_prefill(int M, int pairs, int G, const int* device_clusters, in
   // (fourteen) stages -> four teams and four (twelve), in us: 34816 x 5120 at M = 200 55.8 -> 55.4, 16384 x 5120 at M = 210 28.48 -> 28.43, 5120 x
   // 17408 at M = 209 35.3 -> 34.8; at 128 tokens 16384 x 5120 at M = 112 20.0 -> 19.1, 34816 x 5120 at M = 128 39.4 -> 37.7.
   best.wdepth = kPMaxWD;
-  while (best.wdepth > kPTeams && prefill_smem(best.tn, best.wdepth) > smem_optin) best.wdepth -= kPTeams;
-  best.smem = prefill_smem(best.tn, best.wdepth);
+  while (best.wdepth > kPTeams && prefill_smem(best.pair, best.tn, best.wdepth) > smem_optin) best.wdepth -= kPTeams;
+  best.smem = prefill_smem(best.pair, best.tn, best.wdepth);
   return best;
+}
+
+// The plan of a dense layer with an epilogue whose tokens fit one tile of a CTA alone: as many K splits as find clusters at
+// once. (row tiles of 128; clusters of S CTAs, as many at once as a B200 of 148 SMs runs)
+PrefillPlan plan_single(int M, int row_tiles, int G, const int* device_clusters, int smem_optin) {
+  constexpr int kClusters[kPMaxSplit + 1] = {0, 148, 74, 46, 33};
+  PrefillPlan plan;
+  plan.pair = false;
+  plan.tn = (M + 15) & ~15;
+  for (int S = 2; S <= kPMaxSplit && S <= G; ++S)
+    if (row_tiles <= kClusters[S] && row_tiles <= device_clusters[S]) plan.splits = S;
+  plan.full_tt = M / plan.tn;
+  plan.tiles = row_tiles;
+  plan.clusters = plan.splits > 1 || row_tiles < device_clusters[1] ? row_tiles : device_clusters[1];
+  plan.wdepth = kPMaxWD;
+  while (plan.wdepth > kPTeams && prefill_smem(false, plan.tn, plan.wdepth) > smem_optin) plan.wdepth -= kPTeams;
+  plan.smem = prefill_smem(false, plan.tn, plan.wdepth);
+  return plan;
 }
 
 int table_bytes(int sets) { return kPGather * (kPSetsTN / 2) * 4 + sets * 12 + 16; }
@@ -878,21 +957,21 @@ int w4a16_workspace_free(w4a16_workspace_t* ws) {
 
 namespace w4a16 {
 namespace {
-void cluster_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* at, int warps, int splits, int clusters, int smem) {
-  cfg.gridDim = dim3(2 * splits * clusters);
+void cluster_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* at, int warps, int size, int clusters, int smem) {
+  cfg.gridDim = dim3(size * clusters);
   cfg.blockDim = dim3(warps * 32);
   cfg.dynamicSmemBytes = smem;
   at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = 2 * splits;
+  at[0].val.clusterDim.x = size;
   at[0].val.clusterDim.y = 1;
   at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
 }
 
-// How many clusters of 2 S CTAs (one CTA per SM) the device runs at once, index S; asked for once per device.
+// How many clusters of S tiles' CTAs (one CTA per SM) the device runs at once, index S; asked for once per device.
 // The kernel's shared-memory attribute is set on the way. Returns nullptr (and sets the error) on failure.
-template <int MODE>
+template <int MODE, bool PAIR>
 const int* cluster_slots(int dev, const DeviceInfo* di) {
   struct Slots {
     bool ready = false;
@@ -903,12 +982,12 @@ const int* cluster_slots(int dev, const DeviceInfo* di) {
   std::lock_guard<std::mutex> lk(mu);
   Slots& s = all[dev & 63];
   if (!s.ready) {
-    cudaError_t e = cudaFuncSetAttribute(k_prefill<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, di->smem_optin);
+    cudaError_t e = cudaFuncSetAttribute(k_prefill<MODE, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, di->smem_optin);
     for (int S = 1; S <= kPMaxSplit && e == cudaSuccess; ++S) {
       cudaLaunchConfig_t cfg = {};
       cudaLaunchAttribute at[1];
-      cluster_config(cfg, at, prefill_warps(MODE), S, 1, prefill_smem(kPMaxTN, kPTeams));
-      e = cudaOccupancyMaxActiveClusters(&s.n[S], k_prefill<MODE>, &cfg);
+      cluster_config(cfg, at, prefill_warps(MODE), PAIR ? 2 * S : S, 1, prefill_smem(true, kPMaxTN, kPTeams));
+      e = cudaOccupancyMaxActiveClusters(&s.n[S], k_prefill<MODE, PAIR>, &cfg);
     }
     if (e != cudaSuccess || s.n[1] < 1) {
       fail(W4A16_ECUDA, "gemm_prefill: the device runs no CTA pair of the kernel (%s)", cudaGetErrorString(e));
@@ -926,7 +1005,7 @@ template <int MODE>
 int current_plan(PrefillPlan& plan, int M, int row_tiles, int layer_tiles, int G) {
   const DeviceInfo* di = device_info();
   if (!di) return W4A16_ECUDA;
-  const int* slots = cluster_slots<MODE>(di->device, di);
+  const int* slots = cluster_slots<MODE, true>(di->device, di);
   if (!slots) return W4A16_ECUDA;
   plan = plan_prefill(M, (layer_tiles + 1) / 2, G, slots, di->smem_optin, 0);
   if (row_tiles < layer_tiles && plan.tn > 0)
@@ -960,11 +1039,11 @@ int encode_acts(CUtensorMap* map, const uint16_t* A, int K, int tokens, int rows
 }
 
 // The launch, programmatic unless a weight write is in front of a kernel that reads weights before its wait.
-template <int MODE>
+template <int MODE, bool PAIR>
 int enqueue_prefill(const PrefillParams& p, const PrefillPlan& plan, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute at[2];
-  cluster_config(cfg, at, prefill_warps(MODE), plan.splits, plan.clusters, plan.smem);
+  cluster_config(cfg, at, prefill_warps(MODE), PAIR ? 2 * plan.splits : plan.splits, plan.clusters, plan.smem);
   const bool behind_write = MODE != kSets && take_weight_write(stream);
   if (!behind_write && pdl_enabled()) {
     // (behind a weight write the launch is fully ordered: the weights are read before the wait)
@@ -973,7 +1052,7 @@ int enqueue_prefill(const PrefillParams& p, const PrefillPlan& plan, cudaStream_
     cfg.numAttrs = 2;
   }
   cfg.stream = stream;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, k_prefill<MODE>, p);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, k_prefill<MODE, PAIR>, p);
   if (e == cudaSuccess) return W4A16_OK;
   if (behind_write) note_weight_write(stream);
   return fail(W4A16_ECUDA, "gemm_prefill: launch: %s", cudaGetErrorString(e));
@@ -1009,7 +1088,7 @@ int launch_prefill(PrefillParams& p, uint16_t* C, const w4a16_weights_t* w, cons
   for (int q = 0; q < p.npeers; ++q)
     if (reinterpret_cast<uintptr_t>(p.C_peers[q]) & 15) p.wide = 0;
   if (int rc = encode_acts(&p.amap, A, w->in_f, M, plan.tn / 2)) return rc;
-  return enqueue_prefill<kPlain>(p, plan, static_cast<cudaStream_t>(stream));
+  return enqueue_prefill<kPlain, true>(p, plan, static_cast<cudaStream_t>(stream));
 }
 }  // namespace
 
@@ -1027,28 +1106,39 @@ int launch_prefill_ragged(const RaggedCall& c, cudaStream_t stream) {
   p.pairs = (p.row_tiles + 1) / 2;
   p.status = di->status;
   PrefillPlan plan;
-  if (c.offsets == nullptr) {
+  const bool sets = c.offsets != nullptr;
+  // Few tokens: a CTA alone per tile. The MMAs of a pair take some 70 cycles each however few the tokens, 560 per k group; a CTA's own
+  // 45, and the expansion of its weights some 450 per group becomes the limit. MEASURED
+  const bool single = sets ? c.slots <= static_cast<long long>(kPSingleMean) * c.sets : c.slots <= kPSingleTN;
+  if (!sets && single) {
+    const int* slots = cluster_slots<kDense, false>(di->device, di);
+    if (!slots) return W4A16_ECUDA;
+    plan = plan_single(c.slots, p.row_tiles, c.G, slots, di->smem_optin);
+  } else if (!sets) {
     if (int rc = current_plan<kDense>(plan, c.slots, p.row_tiles, p.row_tiles, c.G)) return rc;
   } else {
-    const int* slots = cluster_slots<kSets>(di->device, di);
+    const int* slots = single ? cluster_slots<kSets, false>(di->device, di) : cluster_slots<kSets, true>(di->device, di);
     if (!slots) return W4A16_ECUDA;
     // Tiles of up to 160 tokens, whatever the sets' sizes: as wide as an expansion pays for (4 TN cycles against some 650), while
     // sets of any size are cut evenly. 64 experts 2048 x 5120, rows in slot order, TN = 64 / 96 / 128 / 160 / 192 / 224: at 300 slots
     // per 8 experts 155 / 144 / 140 / 131 / 131 / 133 us, at 4096 904 / 699 / 600 / 562 / 573 / 611.
-    plan.tn = kPSetsTN;
+    plan.pair = !single;
+    plan.tn = single ? kPSingleTN : kPSetsTN;
     plan.clusters = slots[1];
     plan.wdepth = kPMaxWD;
-    while (plan.wdepth > kPTeams && prefill_smem(plan.tn, plan.wdepth) + table_bytes(c.sets) > di->smem_optin) plan.wdepth -= kPTeams;
-    plan.smem = prefill_smem(plan.tn, plan.wdepth) + table_bytes(c.sets);
+    while (plan.wdepth > kPTeams && prefill_smem(plan.pair, plan.tn, plan.wdepth) + table_bytes(c.sets) > di->smem_optin) plan.wdepth -= kPTeams;
+    plan.smem = prefill_smem(plan.pair, plan.tn, plan.wdepth) + table_bytes(c.sets);
     W4_REQUIRE(plan.smem <= di->smem_optin, "experts_linear: %d bytes of shared memory", plan.smem);
   }
+  if (single) p.pairs = p.row_tiles;
   p.tn = plan.tn;
   p.splits = plan.splits;
   p.wdepth = plan.wdepth;
   p.full_tt = plan.full_tt;
   p.tiles = plan.tiles;
-  if (int rc = encode_acts(&p.amap, c.x, c.K, c.x_tokens, c.x_rows ? 1 : plan.tn / 2)) return rc;
-  return c.offsets ? enqueue_prefill<kSets>(p, plan, stream) : enqueue_prefill<kDense>(p, plan, stream);
+  if (int rc = encode_acts(&p.amap, c.x, c.K, c.x_tokens, c.x_rows ? 1 : single ? plan.tn : plan.tn / 2)) return rc;
+  if (single) return sets ? enqueue_prefill<kSets, false>(p, plan, stream) : enqueue_prefill<kDense, false>(p, plan, stream);
+  return sets ? enqueue_prefill<kSets, true>(p, plan, stream) : enqueue_prefill<kDense, true>(p, plan, stream);
 }
 }  // namespace w4a16
 
