@@ -67,7 +67,8 @@ constexpr int kPBars = 2 * kPMaxWD + kPDone + kPMaxA + kPSteps + 2;
 // Tensor memory: the accumulator's TN columns, the rest are slots of the A operand, 64 columns per k group.
 __host__ __device__ constexpr int a_slots(int tn) { return tn <= 128 ? 6 : 4; }
 constexpr int kPSetsTN = 160;               // tokens of a tile with sets
-constexpr int kPSingleTN = 80, kPSingleMean = 48;  // tokens of a tile of a CTA alone at most; mean set up to which sets take such
+constexpr int kPSingleTN = 80;                // tokens of a tile of a CTA alone at most
+constexpr int kPSingleMean = 24, kPSingleGathered = 10;  // mean set up to which sets take such tiles
 static_assert(kPSingleTN <= kPSetsTN / 2, "lists of rows");
 static_assert(128 + 6 * 64 <= 512 && 256 + 4 * 64 <= 512 && kPMaxA <= kPDone && kPSteps <= kPDone, "ring depths");
 
@@ -1107,9 +1108,11 @@ int launch_prefill_ragged(const RaggedCall& c, cudaStream_t stream) {
   p.status = di->status;
   PrefillPlan plan;
   const bool sets = c.offsets != nullptr;
-  // Few tokens: a CTA alone per tile. The MMAs of a pair take some 70 cycles each however few the tokens, 560 per k group; a CTA's own
-  // 45, and the expansion of its weights some 450 per group becomes the limit. MEASURED
-  const bool single = sets ? c.slots <= static_cast<long long>(kPSingleMean) * c.sets : c.slots <= kPSingleTN;
+  // Few tokens: a CTA alone per tile. It has no hand-over to another CTA, and twice as many tiles to share out; for it every CTA brings in all
+  // of the tile's tokens, in the sets' gathered loads sooner than pays. us, pair / alone: 34816 x 5120 at M = 9 29.6 / 27.9, at 64 32.5 / 31.6, at 77
+  // 33.5 / 32.8; 2048 x 2048 at M = 9 6.4 / 4.0; 64 experts of 8 picks, 2048 x 5120 gathered, at 64 / 128 / 200 tokens 101 / 103 / 112 and 99 / 108 / 120,
+  // 5120 x 1024 in slot order 67 / 70 / 71 and 63 / 67 / 69, at 300 73.8 and 74.8.
+  const bool single = sets ? c.slots <= static_cast<long long>(c.x_rows ? kPSingleGathered : kPSingleMean) * c.sets : c.slots <= kPSingleTN;
   if (!sets && single) {
     const int* slots = cluster_slots<kDense, false>(di->device, di);
     if (!slots) return W4A16_ECUDA;
