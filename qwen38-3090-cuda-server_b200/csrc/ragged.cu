@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(kRThreads, 2) k_ragged(const __grid_constant__
     fence_mbar_init();
   }
   pdl_launch_dependents();
-  pdl_wait();  // offsets, rows and activations come from the kernels in front
+  if (c.offsets) pdl_wait();  // offsets, and with them everything else, come from the kernels in front
   if (warp == 0) {
     // units of every set: ceil(tokens / NT) chunks of each row tile
     int run = 0;
@@ -195,21 +195,37 @@ __global__ void __launch_bounds__(kRThreads, 2) k_ragged(const __grid_constant__
     for (int u = cluster; !dead && u < units; u += nclusters) {
       const Unit t = unit_of<NT>(u, e, first, bounds, c.sets);
       const uint8_t* src = c.stream + static_cast<size_t>(t.e) * c.set_bytes + (static_cast<size_t>(t.rt) * c.G + g0) * kTileGroupBytes;
+      // The ring is empty for the first unit: its first stages' weights are on their way before the tokens' rows are known, and, where
+      // they do not depend on the kernel in front (one set), before that has ended.
+      int early = 0;
+      if (u == cluster) {
+        early = min(p.depth, (g1 - g0 + kRGroups - 1) / kRGroups);
+        if (lane == 0)
+          for (int i = 0; i < early; ++i) {
+            const uint32_t ng = min(kRGroups, g1 - g0 - i * kRGroups);
+            mbar_expect_tx(full_a + i * 8, ng * (kTileGroupBytes + t.n * kGroup * 2));
+            bulk_g2s(ring_a + i * stage_bytes<NT>(), src + i * kRGroups * kTileGroupBytes, ng * kTileGroupBytes, full_a + i * 8);
+          }
+        __syncwarp();
+        if (!c.offsets) pdl_wait();
+      }
       int row = t.slot0 + min(lane, t.n - 1);
       if (c.x_rows) row = __ldcg(c.x_rows + row);
       row = min(max(row, 0), c.x_tokens - 1);  // (no read outside x, whatever the rows hold)
       const uint16_t* xr = c.x + static_cast<size_t>(row) * c.K + static_cast<size_t>(g0) * kGroup;
       for (int g = g0; g < g1; g += kRGroups, src += kRGroups * kTileGroupBytes, xr += kRGroups * kGroup) {
-        if (!warp_agrees(mbar_wait_bounded_relaxed(empty_a + st * 8, ph, kRSpin))) {
-          dead = true;
-          break;
-        }
         const uint32_t dst = ring_a + st * stage_bytes<NT>(), ng = min(kRGroups, g1 - g);
-        if (lane == 0) {
-          mbar_expect_tx(full_a + st * 8, ng * (kTileGroupBytes + t.n * kGroup * 2));
-          bulk_g2s(dst, src, ng * kTileGroupBytes, full_a + st * 8);
+        if (--early < 0) {
+          if (!warp_agrees(mbar_wait_bounded_relaxed(empty_a + st * 8, ph, kRSpin))) {
+            dead = true;
+            break;
+          }
+          if (lane == 0) {
+            mbar_expect_tx(full_a + st * 8, ng * (kTileGroupBytes + t.n * kGroup * 2));
+            bulk_g2s(dst, src, ng * kTileGroupBytes, full_a + st * 8);
+          }
+          __syncwarp();
         }
-        __syncwarp();
         if (lane < t.n) bulk_g2s(dst + kRGroups * kTileGroupBytes + lane * kXPitch, xr, ng * kGroup * 2, full_a + st * 8);
         ++issued;
         if (++st == p.depth) {
@@ -307,6 +323,7 @@ __global__ void __launch_bounds__(kRThreads, 2) k_ragged(const __grid_constant__
         ph ^= 1;
       }
     }
+    if (!c.offsets) pdl_wait();  // bias and residual, and y's readers, may be in the kernel in front
     // ---- the halves' (and the splits') sums meet in shared memory; every output is added up in one order and finished by one thread
     named_bar_sync(1, kRCons * 32);  // the unit before has been read out
 #pragma unroll
@@ -437,13 +454,17 @@ int launch_ragged(RaggedParams& p, const DeviceInfo* di, int max_units, cudaStre
     at[0].val.clusterDim.z = 1;
     cfg.numAttrs = 1;
   }
-  if (pdl_enabled()) {
+  // (behind a weight write the launch of one set is fully ordered: its weights are read before the wait)
+  const bool behind_write = p.c.offsets == nullptr && take_weight_write(st);
+  if (!behind_write && pdl_enabled()) {
     at[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
     ++cfg.numAttrs;
   }
   const cudaError_t err = cudaLaunchKernelEx(&cfg, k_ragged<NT>, p);
-  return err == cudaSuccess ? W4A16_OK : fail(W4A16_ECUDA, "linear: launch: %s", cudaGetErrorString(err));
+  if (err == cudaSuccess) return W4A16_OK;
+  if (behind_write) note_weight_write(st);
+  return fail(W4A16_ECUDA, "linear: launch: %s", cudaGetErrorString(err));
 }
 
 bool aligned16(const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; }
