@@ -255,7 +255,7 @@ int w4a16_experts_view(const w4a16_experts_t* w, int expert, w4a16_weights_t* vi
  *           device; bounds and rows outside these ranges are clamped into them, so that no call leaves its buffers, but what
  *           it then writes into y is not specified.
  *   bias    bf16 [num_experts][out_f] or NULL; activation, precision and alignment as in w4a16_linear_epilogue.
- * Experts without slots cost nothing. One launch. y must not overlap x or bias. */
+ * Experts without slots cost nothing. One launch. y must not overlap x, bias, offsets or x_rows. */
 int w4a16_experts_linear(uint16_t* y, const w4a16_experts_t* w, const uint16_t* x, int x_tokens, const int32_t* x_rows,
                          const int32_t* offsets, int slots, const uint16_t* bias, int activation, void* stream);
 /* Router: of each token's num_experts logits (fp32 or bf16, [T][num_experts]) the top_k largest (1..16), ties to the lowest index.
@@ -272,7 +272,8 @@ int w4a16_route(int32_t* ids, float* weights, int32_t* offsets, int32_t* slots, 
                 int T, int num_experts, int top_k, int renormalize, void* workspace, size_t workspace_bytes, void* stream);
 /* The experts' outputs back to their tokens: y[t] = residual[t] + sum over j of weights[t][j] * parts[slots[t][j]], summed in fp32 in
  * the order of j and rounded once. Picks whose slot is not in [0, parts_rows) count as empty. parts bf16 [parts_rows][hidden],
- * y and residual (may be NULL, may be y itself) bf16 [T][hidden], all 16-byte aligned; hidden a multiple of 8, top_k 1..16. */
+ * y and residual (may be NULL, may be y itself) bf16 [T][hidden], all 16-byte aligned; hidden a multiple of 8, top_k 1..16. y must not
+ * overlap parts, slots or weights. */
 int w4a16_experts_combine(uint16_t* y, const uint16_t* parts, int parts_rows, const int32_t* slots, const float* weights,
                           const uint16_t* residual, int T, int top_k, int hidden, void* stream);
 

@@ -42,6 +42,7 @@
 #include <cuda.h>
 #include <cstring>
 #include <mutex>
+#include <type_traits>
 
 #include "ragged.cuh"
 
@@ -105,7 +106,7 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 template <bool PAIR>  // the pair leader's barrier (a mapped address), or this CTA's own
-__device__ __forceinline__ void arrive_at(uint32_t bar) {
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar, std::bool_constant<PAIR>) {
   if constexpr (PAIR)
     mbar_arrive_cluster(bar);
   else
@@ -303,6 +304,7 @@ __device__ __forceinline__ void finish_four(const RaggedCall& c, int N, int tok,
 template <int MODE, bool PAIR>
 __global__ void __launch_bounds__(prefill_warps(MODE) * 32, 1) k_prefill(const __grid_constant__ PrefillParams p) {
   constexpr int CG = PAIR ? 2 : 1;  // CTAs of a tile
+  constexpr std::bool_constant<PAIR> pair{};
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -636,7 +638,7 @@ __global__ void __launch_bounds__(prefill_warps(MODE) * 32, 1) k_prefill(const _
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) arrive_at<PAIR>(afull_l + a * 8);
+      if (lane == 0) mbar_arrive_cluster(afull_l + a * 8, pair);
       if ((a += kPTeams) >= na) a -= na;
       if ((st += kPTeams) >= WD) {
         st -= WD;
@@ -688,7 +690,7 @@ __global__ void __launch_bounds__(prefill_warps(MODE) * 32, 1) k_prefill(const _
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) arrive_at<PAIR>(dempty_l);
+        if (lane == 0) mbar_arrive_cluster(dempty_l, pair);
       }
       named_bar_sync(1, EW * 32);  // every epilogue warp comes here for every tile, dead or not
       if (cl < cols && !dead)
@@ -720,7 +722,7 @@ __global__ void __launch_bounds__(prefill_warps(MODE) * 32, 1) k_prefill(const _
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) arrive_at<PAIR>(dempty_l);
+        if (lane == 0) mbar_arrive_cluster(dempty_l, pair);
       }
       named_bar_sync(1, EW * 32);  // every epilogue warp comes here for every tile, dead or not
       const int r0 = (CG * t.pair + half) * kTileRows;

@@ -248,8 +248,8 @@ __global__ void __launch_bounds__(kRThreads, 2) k_ragged(const __grid_constant__
 
   if (warp == kRCons + 1) {
     // ================================================================ the rows' constants
-    // Every lane of eight consumer lanes needs the same ones: made once, read by 16-byte loads. 34816 x 5120 at M = 1
-    // In place of eight small loads and eight permutes per lane and group: 1460 instructions per weight block instead of 1630 (M = 9).
+    // All lanes of a row need the same ones: made once, read by one 16-byte load in place of eight small loads and eight permutes per lane
+    // and group (1460 instructions per weight block instead of 1630, 34816 x 5120 at M = 9).
     uint32_t ph = 0;
     for (int u = cluster; !dead && u < units; u += nclusters) {
       for (int g = g0; g < g1; g += kRGroups) {
@@ -274,9 +274,7 @@ __global__ void __launch_bounds__(kRThreads, 2) k_ragged(const __grid_constant__
           }
         }
         large = __any_sync(0xffffffffu, large);
-        if (lane == 0) {
-          sts32(blk + large_offset<NT>(), large);
-        }
+        if (lane == 0) sts32(blk + large_offset<NT>(), large);
         __syncwarp();
         if (lane == 0) mbar_arrive(ready_a + st * 8);
         if (++st == p.depth) {
@@ -484,6 +482,9 @@ int run_ragged(RaggedCall& c, const char* who, cudaStream_t st) {
   W4_REQUIRE(ranges_apart(c.x, xb, c.y, yb), "%s: y overlaps x", who);
   W4_REQUIRE(c.residual == nullptr || c.residual == c.y || ranges_apart(c.residual, yb, c.y, yb), "%s: residual overlaps y but is not y", who);
   W4_REQUIRE(c.bias == nullptr || ranges_apart(c.bias, static_cast<size_t>(c.sets) * c.N * 2, c.y, yb), "%s: y overlaps bias", who);
+  W4_REQUIRE(ranges_apart(c.offsets, c.offsets ? static_cast<size_t>(c.sets + 1) * 4 : 0, c.y, yb) &&
+                 ranges_apart(c.x_rows, c.x_rows ? static_cast<size_t>(c.slots) * 4 : 0, c.y, yb),
+             "%s: y overlaps offsets or x_rows", who);
   const DeviceInfo* di = device_info();
   if (!di) return W4A16_ECUDA;
   RaggedParams p = {};

@@ -329,7 +329,7 @@ int enqueue(Kernel kernel, dim3 grid, int threads, const Params& p, void* stream
   return e == cudaSuccess ? W4A16_OK : fail(W4A16_ECUDA, "%s: launch: %s", who, cudaGetErrorString(e));
 }
 
-int route_blocks(int T) { return (T + kRouteWarps - 1) / kRouteWarps; }
+int route_blocks(int T) { return T / kRouteWarps + (T % kRouteWarps != 0); }
 
 }  // namespace
 }  // namespace w4a16
@@ -396,6 +396,9 @@ int w4a16_experts_combine(uint16_t* y, const uint16_t* parts, int parts_rows, co
   const size_t yb = static_cast<size_t>(T) * hidden * 2;
   W4_REQUIRE(ranges_apart(parts, static_cast<size_t>(parts_rows) * hidden * 2, y, yb), "experts_combine: y overlaps parts");
   W4_REQUIRE(residual == nullptr || residual == y || ranges_apart(residual, yb, y, yb), "experts_combine: residual overlaps y but is not y");
+  const size_t picks = static_cast<size_t>(T) * top_k * 4;
+  W4_REQUIRE(ranges_apart(slots, picks, y, yb) && ranges_apart(weights, picks, y, yb), "experts_combine: y overlaps slots or weights");
+  if (parts_rows == 0) parts = y;  // (no row is read, but the copies that fill empty picks with zeros name an address)
   const DeviceInfo* di = device_info();
   if (!di) return W4A16_ECUDA;
   const uint32_t strips = (static_cast<uint32_t>(hidden) + 255) / 256;

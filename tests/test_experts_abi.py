@@ -1,6 +1,8 @@
 """Refusals of the feed-forward operators that the library makes before it touches a device, and the sizes it states."""
 import ctypes as C
 
+import test_ring_handback
+
 
 def _weights(pkg, rows=128, cols=256):
     w = pkg.Weights()
@@ -14,6 +16,12 @@ def _experts(pkg, **fields):
     for name, v in fields.items():
         setattr(w, name, v)
     return w
+
+
+def test_one_lane_arrives_behind_a_syncwarp(monkeypatch):
+    monkeypatch.setattr(test_ring_handback, "HANDED_OVER", ("ready_a", "empty_a"))
+    seen = list(test_ring_handback._arrivals("ragged.cu"))
+    assert [bar for _, bar, _ in seen] == ["ready_a", "empty_a"] and all(before == "__syncwarp();" for *_, before in seen)
 
 
 def test_struct_layout(pkg):
@@ -69,6 +77,8 @@ def test_experts_refusals(pkg):
     assert call(act=9) == -1
     assert call(w=_experts(pkg, num_experts=0)) == -1 and call(w=_experts(pkg, num_groups=3)) == -1
     assert call(w=_experts(pkg, out_f=112), act=4) == -1
+    assert call(offsets=(1 << 20) + 16) == -1 and b"overlaps offsets" in L.w4a16_last_error()
+    assert call(rows=(1 << 20) - 28) == -1 and b"x_rows" in L.w4a16_last_error()
 
 
 def test_route_and_combine_refusals(pkg):
@@ -89,8 +99,9 @@ def test_route_and_combine_refusals(pkg):
         assert route(**{name: p + 2}) == -1
     assert route(logits=p + 1, f32=0) == -1
     assert route(T=33, nbytes=2 * 8 * 4) == -3 and route(T=33, ws=None) == -3
+    assert L.w4a16_route_workspace(2 ** 31 - 1, 8) == (2 ** 26 + 1) * 8 * 4 and route(T=2 ** 31 - 1, k=1) == -3
 
-    def combine(y=p, parts=1 << 24, n=8, slots=p, weights=p, residual=None, T=4, k=2, H=64):
+    def combine(y=p, parts=1 << 24, n=8, slots=1 << 26, weights=1 << 27, residual=None, T=4, k=2, H=64):
         return L.w4a16_experts_combine(y, parts, n, slots, weights, residual, T, k, H, None)
 
     assert combine(T=0) == 0
@@ -99,3 +110,5 @@ def test_route_and_combine_refusals(pkg):
     assert combine(y=None) == -1 and combine(slots=None) == -1 and combine(weights=None) == -1 and combine(parts=None) == -1
     assert combine(y=p + 8) == -1 and combine(parts=(1 << 24) + 2) == -1 and combine(slots=p + 2) == -1
     assert combine(parts=p + 4 * 64 * 2 - 16) == -1 and combine(residual=p + 16) == -1
+    assert combine(slots=p - 4) == -1 and b"overlaps slots" in L.w4a16_last_error()
+    assert combine(weights=p + 508) == -1 and b"overlaps slots" in L.w4a16_last_error()

@@ -85,6 +85,54 @@ def test_activations(pkg, act, bias, counts):
     _check(pkg, counts, 352, 512, act=act, bias=bias)
 
 
+@pytest.mark.parametrize("counts", [[3200] + [0] * 400 + [5] * 111, [0] * 511 + [40], [0, 2, 1, 15] * 128, [0] * 511 + [6000], [0, 25, 3, 70] * 128])
+@pytest.mark.parametrize("gather", [True, False])
+def test_as_many_experts_as_a_container_takes(pkg, counts, gather):
+    """Tables of 512 sets beside each kernel's stages; expert 511's rows."""
+    _check(pkg, counts, 144, 256, gather=gather, bias=True, spare=2)
+
+
+@pytest.mark.parametrize("n", [3, 40, 3500])
+def test_experts_past_four_gigabytes_of_weights(pkg, n):
+    E, rows, cols = 512, 34816, 512
+    w = pkg.experts_alloc(E, rows, cols)
+    t = disk(rows, cols, 5)
+    pkg.awq_repack_into(pkg.experts_view(w, E - 1), 0, *t)
+    x = whole((n, cols), 4, 1)
+    y = torch.empty((n, rows), dtype=torch.bfloat16, device="cuda")
+    pkg.experts_linear(y, w, x, torch.tensor([0] * E + [n], dtype=torch.int32, device="cuda"))
+    assert torch.equal(y, (x.double() @ weights64(*t).T).to(torch.bfloat16))
+    pkg.experts_free(w)
+
+
+@pytest.mark.parametrize("gather", [True, False])
+def test_rows_past_four_gigabytes(pkg, gather):
+    """Inputs and outputs whose offsets pass 32 bits, in bytes and in elements."""
+    n, tokens, K, N = 140000, 80, 128, 17408
+    bank = Bank(pkg, 3, N, K)
+    at, offsets = _offsets([n - 50, 0, 50])
+    x = whole((tokens if gather else n, K), 4, 1)
+    rows = (torch.arange(n, dtype=torch.int32, device="cuda") % tokens) if gather else None
+    y = torch.empty((n, N), dtype=torch.bfloat16, device="cuda")
+    pkg.experts_linear(y, bank.w, x, offsets, x_rows=rows)
+    for e, lo, hi in ((0, 0, 300), (0, n - 400, n - 50), (2, n - 50, n)):
+        xe = x[rows[lo:hi].long()] if gather else x[lo:hi]
+        assert torch.equal(y[lo:hi], bank.layer64(e, xe).to(torch.bfloat16))
+    # and as inputs: the last rows, of 17408 columns
+    back = Bank(pkg, 3, 128, N, seed=1)
+    y[n - 400:].copy_(whole((400, N), 4, 2))
+    last = torch.arange(n - 1, n - 41, -1, dtype=torch.int32, device="cuda")
+    z = torch.empty((40, 128), dtype=torch.bfloat16, device="cuda")
+    off = torch.tensor([0, 0, 30, 40], dtype=torch.int32, device="cuda")
+    for count in (12, 40):  # few rows and many
+        pkg.experts_linear(z[:count], back.w, y, off.clamp(max=count), x_rows=last[:count])
+        for e, lo, hi in ((1, 0, min(30, count)), (2, 30, 40)):
+            if hi <= count:
+                assert torch.equal(z[lo:hi], back.layer64(e, y[last[lo:hi].long()]).to(torch.bfloat16))
+    bank.free()
+    back.free()
+
+
 def test_no_slots_at_all(pkg):
     _check(pkg, [0, 0, 0], 128, 128, spare=4)
     _check(pkg, [0, 0, 0], 128, 128)
@@ -138,6 +186,25 @@ def test_a_view_is_a_layer_of_its_own(pkg):
     with pytest.raises(pkg.W4A16Error):
         pkg.experts_view(bank.w, 3)
     bank.free()
+
+
+@pytest.mark.parametrize("counts", [[2, 0, 1], [50, 0, 30]])
+def test_right_behind_a_repack(pkg, counts):
+    """Experts repacked on the same stream without a wait in between, read as a group and by themselves."""
+    E, rows, cols = 3, 1024, 512
+    w = pkg.experts_alloc(E, rows, cols)
+    at, offsets = _offsets(counts)
+    x = whole((at[-1], cols), 4, 1)
+    y, z = torch.empty((at[-1], rows), dtype=torch.bfloat16, device="cuda"), torch.empty((counts[2], rows), dtype=torch.bfloat16, device="cuda")
+    for seed in range(30, 50, 4):
+        tensors = [disk(rows, cols, seed + e) for e in range(E)]
+        for e, t in enumerate(tensors):
+            pkg.awq_repack_into(pkg.experts_view(w, e), 0, *t)
+        pkg.experts_linear(y, w, x, offsets)
+        pkg.linear_epilogue(z, pkg.experts_view(w, 2), x[at[2]:], counts[2])
+        want = torch.cat([x[at[e]:at[e + 1]].double() @ weights64(*t).T for e, t in enumerate(tensors)]).to(torch.bfloat16)
+        assert torch.equal(y, want) and torch.equal(z, want[at[2]:])
+    pkg.experts_free(w)
 
 
 # ------------------------------------------------------------------ router
@@ -260,6 +327,19 @@ def test_combine(pkg, T, k, H, residual):
     pkg.experts_combine(out.t, parts, slots, weights, residual=r)
     assert out.intact()
     assert bool(((out.t.double() - ref).abs() <= ref.abs() * 2.0 ** -8 + mass * ((k + 1) * 2.0 ** -24)).all())
+
+
+def test_combine_past_four_gigabytes(pkg):
+    T, H = 450000, 5120
+    parts = torch.empty((T, H), dtype=torch.bfloat16, device="cuda")
+    parts[:9], parts[-9:] = whole((9, H), 4, 1), whole((9, H), 4, 2)
+    slots = torch.full((T, 2), -1, dtype=torch.int32, device="cuda")
+    slots[-4:] = torch.tensor([[0, T - 1], [T - 2, T - 9], [8, -1], [T - 3, T]], dtype=torch.int32)
+    y = torch.empty((T, H), dtype=torch.bfloat16, device="cuda")
+    pkg.experts_combine(y, parts, slots, torch.ones((T, 2), device="cuda"))
+    p = parts[[0, T - 1, T - 2, T - 9, 8, T - 3]].float()
+    assert torch.equal(y[-4:].float(), torch.stack([p[0] + p[1], p[2] + p[3], p[4], p[5]]))
+    assert int(torch.count_nonzero(y[:-4])) == 0
 
 
 def test_combine_empty_picks_read_nothing(pkg):

@@ -5,6 +5,7 @@ import torch
 
 from ffn_util import activate64, assert_close_to_rounding, code, disk, weights64, whole
 from gpu_util import Guarded
+from test_gpu_prefill_tiles import _one_weight_per_output
 
 pytestmark = pytest.mark.gpu
 
@@ -125,6 +126,31 @@ def test_large_gates_and_infinite_residuals(pkg):
         pkg.linear_epilogue(y, w, x, 2, activation=act, residual=r)
         assert bool((y[1] == 0).all()) and float(y[0, 3]) == -float("inf")
         assert bool((torch.cat([y[0, :3], y[0, 4:]]) == 3840).all())
+    pkg.awq_free(w)
+
+
+@pytest.mark.parametrize("M", [1, 8, 16, 77, 300])
+def test_every_weight_by_itself(pkg, synth, M):
+    """Scales of every kind (subnormal, largest, either sign), every code and zero point, and one power of two per token: an output is one
+    weight times it, exactly, wherever that is a normal number."""
+    N, K = 272, 384
+    q, z, scale = _one_weight_per_output(N, K, seed=M)
+    w = pkg.weights_from_numpy(synth.pack_weight(q), scale, synth.pack_zero_point(z))
+    want = torch.empty((N, K), dtype=torch.bfloat16, device="cuda")
+    pkg.w4a16_dequant_rows(want, w, 0, N)
+    want = want.double()
+    y = torch.empty((M, N), dtype=torch.bfloat16, device="cuda")
+    for power in (2.0 ** 60, 2.0 ** -60):
+        for k0 in range(0, K, M) if M > 1 else (0, 127, 128, 255, 383):
+            n = min(M, K - k0)
+            x = torch.zeros((M, K), dtype=torch.bfloat16, device="cuda")
+            x[torch.arange(n), torch.arange(k0, k0 + n)] = power
+            pkg.linear_epilogue(y, w, x, M)
+            got, ref = y[:n].double().t(), want[:, k0:k0 + n] * power
+            normal = (ref.abs() >= 2.0 ** -126) & (ref.abs() < 2.0 ** 128)
+            assert torch.equal(got[normal], ref[normal])
+            assert bool((got[ref == 0] == 0).all())
+    assert pkg.device_status() == 0
     pkg.awq_free(w)
 
 
