@@ -67,7 +67,8 @@ constexpr int kPMaxA = 6;                   // A slots, at most
 constexpr int kPBars = 2 * kPMaxWD + kPDone + kPMaxA + kPSteps + 2;
 // Tensor memory: the accumulator's TN columns, the rest are slots of the A operand, 64 columns per k group.
 __host__ __device__ constexpr int a_slots(int tn) { return tn <= 128 ? 6 : 4; }
-constexpr int kPSetsTN = 160;               // tokens of a tile with sets
+constexpr int kPSetsTN = 224, kPSetsNarrow = 128;  // tokens of a tile with sets, and with small ones:
+constexpr int kPSetsMean = 64;                     // mean set up to which the narrow tile is taken
 constexpr int kPSingleTN = 80;                // tokens of a tile of a CTA alone at most
 constexpr int kPSingleMean = 24, kPSingleGathered = 10;  // mean set up to which sets take such tiles
 static_assert(kPSingleTN <= kPSetsTN / 2, "lists of rows");
@@ -208,7 +209,7 @@ __device__ __forceinline__ PTile tile_of(const PrefillParams& p, int tile) {
 }
 
 // Sets: their slots and the tiles in front of each, in shared memory. A set's tokens are cut into equal tiles (a multiple of 32, at
-// most TN): up to some 160 tokens a tile costs its expansion, whatever it multiplies.
+// most TN), which all expand the set's weights.
 struct SetTable {
   const int2* bounds;
   const int* first;  // [sets + 1]
@@ -1124,11 +1125,15 @@ int launch_prefill_ragged(const RaggedCall& c, cudaStream_t stream) {
   } else {
     const int* slots = single ? cluster_slots<kSets, false>(di->device, di) : cluster_slots<kSets, true>(di->device, di);
     if (!slots) return W4A16_ECUDA;
-    // Tiles of up to 160 tokens, whatever the sets' sizes: as wide as an expansion pays for (4 TN cycles against some 650), while
-    // sets of any size are cut evenly. 64 experts 2048 x 5120, rows in slot order, TN = 64 / 96 / 128 / 160 / 192 / 224: at 300 slots
-    // per 8 experts 155 / 144 / 140 / 131 / 131 / 133 us, at 4096 904 / 699 / 600 / 562 / 573 / 611.
+    // A set is cut into equal tiles of up to 224 tokens, the most whose stages fit: every tile expands the set's weights anew, which costs
+    // time up to some 160 tokens (4 TN cycles of MMA against some 650) and power, the limit of a long launch, beyond. Sets that mostly
+    // fit 128 take that, which leaves room for six slots of the A operand and three times the weight stages. us in loops of half a second, 160 / 192 / 224: 64
+    // experts of 8 picks, 2048 x 5120 gathered, at 300 tokens 128.0 / 127.9 / 128.5, 600 169.7 / 174.1 / 166.6, 800 199 / 195 / 195, 1400 281 / 270 / 262, 3000
+    // 514 / 504 / 482, 8192 1295 / 1250 / 1194; 5120 x 1024 in slot order 79.0 / 79.6 / 81.0, 95.7 / 95.9 / 97.2, 111 / 110 / 109, 158 / 152 / 150, 283 / 277 /
+    // 273, 713 / 689 / 682. In short runs, 160 / 128: 300 tokens 119.5 / 117.9 and 71.9 / 71.1, 450 134.0 / 132.6 and 76.6 / 76.7, 600 149.3 / 148.7 and 81.6 / 84.1.
+    // (Two accumulators of 128 columns, so that a tile is read out under the next one's main loop, gave 1 % at most.)
     plan.pair = !single;
-    plan.tn = single ? kPSingleTN : kPSetsTN;
+    plan.tn = single ? kPSingleTN : c.slots <= static_cast<long long>(kPSetsMean) * c.sets ? kPSetsNarrow : kPSetsTN;
     plan.clusters = slots[1];
     plan.wdepth = kPMaxWD;
     while (plan.wdepth > kPTeams && prefill_smem(plan.pair, plan.tn, plan.wdepth) + table_bytes(c.sets) > di->smem_optin) plan.wdepth -= kPTeams;
