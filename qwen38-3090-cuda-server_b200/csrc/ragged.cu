@@ -82,7 +82,7 @@ __host__ __device__ constexpr int stage_bytes() {
   return large_offset<NT>() + 16;
 }
 template <int NT>
-__host__ __device__ constexpr int sum_bytes() {  // the two k halves' sums: [2][NT tokens][128 rows] floats
+__host__ __device__ constexpr int sum_bytes() {  // the two k halves' sums, [2][NT tokens][128 rows] floats, or one half's of two units
   return 2 * NT * kTileRows * 4;
 }
 
@@ -301,6 +301,7 @@ __global__ void __launch_bounds__(kRThreads, 2) k_ragged(const __grid_constant__
   const uint32_t c_off = consts_offset<NT>() + r0 * 16;
   const uint32_t x_off = kRGroups * kTileGroupBytes + (lane >> 2) * kXPitch + (half * 64 + t4 * 16) * 2;
   uint32_t ph = 0;
+  int parity = 0;
   for (int u = cluster; u < units; u += nclusters) {
     const Unit t = unit_of<NT>(u, e, first, bounds, c.sets);
     float acc[2][NT / 8][4] = {};
@@ -322,32 +323,10 @@ __global__ void __launch_bounds__(kRThreads, 2) k_ragged(const __grid_constant__
       }
     }
     if (!c.offsets) pdl_wait();  // bias and residual, and y's readers, may be in the kernel in front
-    // ---- the halves' (and the splits') sums meet in shared memory; every output is added up in one order and finished by one thread
-    named_bar_sync(1, kRCons * 32);  // the unit before has been read out
-#pragma unroll
-    for (int j = 0; j < NT / 8; ++j)
-      if (j == 0 || 8 * j < t.n)
-#pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            sums[(half * NT + 8 * j + 2 * t4 + (i & 1)) * kTileRows + r0 + 16 * m + 8 * (i >> 1)] = acc[m][j][i];
-    if (S > 1) cluster_sync();
-    named_bar_sync(1, kRCons * 32);
-    const int pairs = t.n * (kTileRows / 2);
-    for (int i = tid + split * kRCons * 32; i < pairs && !dead; i += S * kRCons * 32) {
-      const int tok = i / (kTileRows / 2), r = 2 * (i % (kTileRows / 2)), row = t.rt * kTileRows + r;
-      if (row >= c.N) continue;
-      float v0 = 0.f, v1 = 0.f;
-      for (int s = 0; s < S; ++s) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float* at = sums + (h * NT + tok) * kTileRows + r;
-          const float2 v = S > 1 ? ld_cluster_f32x2(map_to_rank(smem_u32(at), s)) : *reinterpret_cast<const float2*>(at);
-          v0 += v.x;
-          v1 += v.y;
-        }
-      }
+    // ---- the halves' (and the splits') sums are added up in one order, and every output is finished by one thread
+    auto finish = [&](int tok, int r, float v0, float v1) {  // rows r and r + 1 of the tile, r even
+      const int row = t.rt * kTileRows + r;
+      if (row >= c.N || tok >= t.n) return;
       if (c.bias) {
         const uint16_t* b = c.bias + static_cast<size_t>(t.e) * c.N;
         v0 += bf16_bits_to_float(b[bias_index(row, c.N, c.act)]);
@@ -370,8 +349,60 @@ __global__ void __launch_bounds__(kRThreads, 2) k_ragged(const __grid_constant__
         }
         *reinterpret_cast<uint32_t*>(c.y + o) = float_to_bf16_bits(v0) | (static_cast<uint32_t>(float_to_bf16_bits(v1)) << 16);
       }
+    };
+    if (S == 1) {
+      // Two warps share 32 rows. Each hands the other its fragments of 16 and finishes the other 16, through two buffers in turn, so that a
+      // unit needs a single barrier of the two (a buffer is written again behind the next unit's).
+      const uint32_t pair_a = smem_u32(sums) + ((parity * (kRCons / 2) + (warp >> 1)) * (NT / 4) * 32 + lane) * 16;
+      const uint32_t give = pair_a + half * (NT / 8) * 512, take = pair_a + (half ^ 1) * (NT / 8) * 512;
+      parity ^= 1;
+#pragma unroll
+      for (int j = 0; j < NT / 8; ++j)
+        if (j == 0 || 8 * j < t.n)
+          sts128(give + j * 512, __float_as_uint(half ? acc[0][j][0] : acc[1][j][0]), __float_as_uint(half ? acc[0][j][1] : acc[1][j][1]),
+                 __float_as_uint(half ? acc[0][j][2] : acc[1][j][2]), __float_as_uint(half ? acc[0][j][3] : acc[1][j][3]));
+      named_bar_sync(1 + (warp >> 1), 64);
+      if (dead) continue;
+      const int odd = (lane >> 2) & 1;
+#pragma unroll
+      for (int j = 0; j < NT / 8; ++j)
+        if (j == 0 || 8 * j < t.n) {
+          const uint4 u = j ? lds128<512>(take) : lds128<0>(take);
+          const float v[4] = {(half ? acc[1][j][0] : acc[0][j][0]) + __uint_as_float(u.x), (half ? acc[1][j][1] : acc[0][j][1]) + __uint_as_float(u.y),
+                              (half ? acc[1][j][2] : acc[0][j][2]) + __uint_as_float(u.z), (half ? acc[1][j][3] : acc[0][j][3]) + __uint_as_float(u.w)};
+          // a lane has one row and two tokens; it takes its neighbour row's sum of one token for its own of the other
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float got = __shfl_xor_sync(0xffffffffu, odd ? v[2 * h] : v[2 * h + 1], 4);
+            finish(8 * j + 2 * t4 + odd, r0 - odd + 16 * half + 8 * h, odd ? got : v[2 * h], odd ? v[2 * h + 1] : got);
+          }
+        }
+      continue;
     }
-    if (S > 1) break;  // (a cluster takes one unit)
+#pragma unroll
+    for (int j = 0; j < NT / 8; ++j)
+      if (j == 0 || 8 * j < t.n)
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            sums[(half * NT + 8 * j + 2 * t4 + (i & 1)) * kTileRows + r0 + 16 * m + 8 * (i >> 1)] = acc[m][j][i];
+    cluster_sync();
+    const int pairs = t.n * (kTileRows / 2);
+    for (int i = tid + split * kRCons * 32; i < pairs && !dead; i += S * kRCons * 32) {
+      const int tok = i / (kTileRows / 2), r = 2 * (i % (kTileRows / 2));
+      float v0 = 0.f, v1 = 0.f;
+      for (int s = 0; s < S; ++s) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float2 v = ld_cluster_f32x2(map_to_rank(smem_u32(sums + (h * NT + tok) * kTileRows + r), s));
+          v0 += v.x;
+          v1 += v.y;
+        }
+      }
+      finish(tok, r, v0, v1);
+    }
+    break;  // (a cluster takes one unit)
   }
   if (dead && lane == 0) atomicExch(p.status, W4A16_ETIMEOUT);
   __syncwarp();
