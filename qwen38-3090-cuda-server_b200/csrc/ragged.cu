@@ -522,10 +522,12 @@ int run_ragged(RaggedCall& c, const char* who, cudaStream_t st) {
   p.c = c;
   p.row_tiles = (c.N + kTileRows - 1) / kTileRows;
   p.status = di->status;
-  // More than a few tokens per set: whole tiles on tcgen05, whose time hardly depends on their number up to 160 (here every eight
-  // tokens cost 64 mma.sync per weight block, beside 1040 instructions for its expansion). us, here / there: 16384 x 5120 at M = 8
-  // 15.5 / 17.1, at 16 19.0 / 17.3; 64 experts 2048 x 5120 with 4 slots each in the mean 89 / 107, with 8 111 / 107.
-  if (c.offsets ? c.slots > 6LL * c.sets : c.slots > 8) return launch_prefill_ragged(c, st);
+  // More than a few tokens per set: whole tiles on tcgen05, whose time hardly depends on their number up to 128 (here every eight
+  // tokens cost 64 mma.sync per weight block, beside 1040 instructions for its expansion), but which cost more at both ends, so that
+  // short rows of weights stay here longer. us, here / there: 16384 x 5120 at M = 8 15.5 / 17.1, at 16 19.0 / 17.3; 2048 x 5120 in 64 sets of 4.1 in
+  // the mean 87.6 / 97.2, of 5 102 / 97, of 6.5 107 / 99; 2048 x 2048 in 256 of 5.6 145 / 149, of 6.5 152 / 151, of 7.5 163 / 156; 5120 x 1024 in 64
+  // of 5 56.5 / 61.1, of 6.5 62.6 / 62.8, of 8.5 66.6 / 63.5.
+  if (c.offsets ? 2LL * c.slots > (c.G >= 32 ? 9LL : 13LL) * c.sets : c.slots > 8) return launch_prefill_ragged(c, st);
   // chunks of NT tokens at most: every set with tokens has one more than its whole ones
   const int used = c.slots < c.sets ? c.slots : c.sets;
   const int nt = c.slots <= 4LL * c.sets || !c.offsets ? 8 : 16;
