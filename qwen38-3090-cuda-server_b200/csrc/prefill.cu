@@ -26,14 +26,18 @@
 //   * few tiles (short prompts, narrow layers): a cluster of 2 S CTAs splits K S ways; the splits' fp32 tiles
 //     are added through distributed shared memory, always in split order (bitwise reproducible).
 //
+// The same pipeline carries the layers with an epilogue (kDense: bias, activation and residual while the accumulator is read
+// out, in fp32) and the products grouped by expert (kSets: every tile belongs to a set of tokens with weights of its own; rows are
+// gathered four at a time by TMA). For few tokens a CTA works alone (PAIR = false: 128 rows x all of the tile's tokens).
+//
 // What bounds it: long prompts run at the tensor cores' rate under the power cap (256 x 256 x 16 per 128 cycles: 1024
 // cycles per k group; tensor pipe 87 % active over a 4096-token launch), short ones by no single role: a CTA and k group takes
 // 640 to 700 cycles (5120 x 17408 at M = 77: issue slots 52 %, ALU pipe 41 % on average and 52 % on the busiest SM, tensor pipe 43 % of active
 // cycles), where HBM would allow 386.
 // In us, weights cold, against one CTA per tile of 128 x 256 with eight dequant warps (by box and temperature: 2 to 10 %):
 //   34816 x 5120, M = 4096: 1264 -> 922 (1583 TFLOP/s); 5120 x 17408, M = 4096: 698 -> 488 (1497)
-//   34816 x 5120, M = 777:   300 -> 208;                5120 x 8192, M = 777:   110 -> 54
-//   34816 x 5120, M = 77:     73 -> 34;                 5120 x 17408, M = 77:   105 -> 23;     8192 x 5120, M = 77: 45 -> 13
+//   34816 x 5120, M = 777:   300 -> 195;                5120 x 8192, M = 777:   110 -> 49
+//   34816 x 5120, M = 77:     73 -> 32;                 5120 x 17408, M = 77:   105 -> 20.5;   8192 x 5120, M = 77: 45 -> 13
 // and on the way, 34816 x 5120 at M = 4096 on one device: half groups as the unit of every hand-off 1134 (the first shape; the
 // issuing thread is the limit), whole groups 1063, two teams of dequant warps (four since) and C through shared memory 890. A warp's vote on
 // its waits took another 9 % off short prompts (34816 x 5120 at M = 77: 40.8 -> 37.1) by keeping the loops warp-uniform.

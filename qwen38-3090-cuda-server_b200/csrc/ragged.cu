@@ -7,11 +7,18 @@
 // A unit of work is a 128-row tile of a set's weights with up to NT of its tokens (NT = 8 or 16). A CTA takes a unit; where there are
 // few units, a cluster of S CTAs shares one, each a range of k groups, and adds up through distributed shared memory in a
 // fixed order (bitwise reproducible). In a CTA
-//   * one producer warp fills a ring of stages, a k group each: the 8576-byte weight block by one bulk copy (cp.async.bulk), each
-//     token's 128 activations by another, so that rows are gathered in the load;
+//   * one producer warp fills a ring of stages, two k groups each: the two 8576-byte weight blocks by one bulk copy (cp.async.bulk), each
+//     token's 256 activations by another, so that rows are gathered in the load;
+//   * one warp makes what the expansion needs of every row and group (zero point and scale as bf16 pairs) once per stage;
 //   * eight consumer warps take 32 rows x 64 k each: mma.sync m16n8k16 with the weights as the A operand straight from the
 //     expansion. The fragments' k order is free as long as both operands share it, so a lane takes 16 consecutive k of
-//     its row (8 bytes of codes) and of its token (two 16-byte loads).
+//     its row (8 bytes of codes) and of its token (two 16-byte loads). Two warps share 32 rows and add up their halves of K.
+//
+// What bounds it: the expansion's instructions. Two CTAs of an SM take some 500 cycles for a weight block where HBM allows 370: 1460
+// warp instructions at M = 8, of which LOP3, shifts and packed bf16 arithmetic issue at half a scheduler's rate (measured by themselves: 345 cycles without
+// the mma.sync, 408 with). 34816 x 5120 at M = 8 25.1 us (3.7 TB/s), 64 experts 5120 x 1024 at 4.1 slots each 52.8 (3.3 TB/s).
+// Tried beside it, the same or slower: 16 rows x 128 k per warp, three CTAs per SM, loads a step ahead, more accumulators, and A in tensor memory for
+// tcgen05.mma with two CTAs per SM (28.5 us at M = 1 against 25).
 #include <climits>
 #include <cstring>
 #include <mutex>
