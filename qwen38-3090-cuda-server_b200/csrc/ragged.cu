@@ -331,31 +331,38 @@ __global__ void __launch_bounds__(kRThreads, 2) k_ragged(const __grid_constant__
     }
     if (!c.offsets) pdl_wait();  // bias and residual, and y's readers, may be in the kernel in front
     // ---- the halves' (and the splits') sums are added up in one order, and every output is finished by one thread
-    auto finish = [&](int tok, int r, float v0, float v1) {  // rows r and r + 1 of the tile, r even
+    const bool gated = c.act == W4A16_ACT_SWIGLU;
+    struct Beside {
+      float b0, b1, r0, r1;
+    };
+    auto beside = [&](int tok, int r) {  // bias and residual of rows r and r + 1 of the tile, r even
       const int row = t.rt * kTileRows + r;
-      if (row >= c.N || tok >= t.n) return;
+      Beside v = {};
+      if (row >= c.N || tok >= t.n) return v;
       if (c.bias) {
         const uint16_t* b = c.bias + static_cast<size_t>(t.e) * c.N;
-        v0 += bf16_bits_to_float(b[bias_index(row, c.N, c.act)]);
-        v1 += bf16_bits_to_float(b[bias_index(row + 1, c.N, c.act)]);
+        v.b0 = bf16_bits_to_float(b[bias_index(row, c.N, c.act)]);
+        v.b1 = bf16_bits_to_float(b[bias_index(row + 1, c.N, c.act)]);
       }
-      const size_t line = static_cast<size_t>(t.slot0 + tok) * c.ny;
-      if (c.act == W4A16_ACT_SWIGLU) {
-        const size_t o = line + (row >> 1);
-        float v = logistic_times(v0, v0) * v1;
-        if (c.residual) v += bf16_bits_to_float(c.residual[o]);
-        c.y[o] = float_to_bf16_bits(v);
-      } else {
-        const size_t o = line + row;
-        v0 = activate(v0, c.act);
-        v1 = activate(v1, c.act);
-        if (c.residual) {
-          const uint32_t r2 = *reinterpret_cast<const uint32_t*>(c.residual + o);
-          v0 += bf16_bits_to_float(static_cast<uint16_t>(r2));
-          v1 += bf16_bits_to_float(static_cast<uint16_t>(r2 >> 16));
-        }
-        *reinterpret_cast<uint32_t*>(c.y + o) = float_to_bf16_bits(v0) | (static_cast<uint32_t>(float_to_bf16_bits(v1)) << 16);
+      if (c.residual) {
+        const uint16_t* at = c.residual + static_cast<size_t>(t.slot0 + tok) * c.ny + (gated ? row >> 1 : row);
+        const uint32_t r2 = gated ? *at : *reinterpret_cast<const uint32_t*>(at);
+        v.r0 = bf16_bits_to_float(static_cast<uint16_t>(r2));
+        v.r1 = bf16_bits_to_float(static_cast<uint16_t>(r2 >> 16));
       }
+      return v;
+    };
+    auto finish = [&](int tok, int r, float v0, float v1, const Beside& v) {
+      const int row = t.rt * kTileRows + r;
+      if (row >= c.N || tok >= t.n) return;
+      v0 += v.b0;
+      v1 += v.b1;
+      uint16_t* at = c.y + static_cast<size_t>(t.slot0 + tok) * c.ny + (gated ? row >> 1 : row);
+      if (gated)
+        *at = float_to_bf16_bits(logistic_times(v0, v0) * v1 + v.r0);
+      else
+        *reinterpret_cast<uint32_t*>(at) = float_to_bf16_bits(activate(v0, c.act) + v.r0) |
+                                           (static_cast<uint32_t>(float_to_bf16_bits(activate(v1, c.act) + v.r1)) << 16);
     };
     if (S == 1) {
       // Two warps share 32 rows. Each hands the other its fragments of 16 and finishes the other 16, through two buffers in turn, so that a
@@ -368,9 +375,10 @@ __global__ void __launch_bounds__(kRThreads, 2) k_ragged(const __grid_constant__
         if (j == 0 || 8 * j < t.n)
           sts128(give + j * 512, __float_as_uint(half ? acc[0][j][0] : acc[1][j][0]), __float_as_uint(half ? acc[0][j][1] : acc[1][j][1]),
                  __float_as_uint(half ? acc[0][j][2] : acc[1][j][2]), __float_as_uint(half ? acc[0][j][3] : acc[1][j][3]));
+      const int odd = (lane >> 2) & 1, tok0 = 2 * t4 + odd, row0 = r0 - odd + 16 * half;
+      const Beside early[2] = {beside(tok0, row0), beside(tok0, row0 + 8)};  // under way while the warps meet
       named_bar_sync(1 + (warp >> 1), 64);
       if (dead) continue;
-      const int odd = (lane >> 2) & 1;
 #pragma unroll
       for (int j = 0; j < NT / 8; ++j)
         if (j == 0 || 8 * j < t.n) {
@@ -381,7 +389,7 @@ __global__ void __launch_bounds__(kRThreads, 2) k_ragged(const __grid_constant__
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const float got = __shfl_xor_sync(0xffffffffu, odd ? v[2 * h] : v[2 * h + 1], 4);
-            finish(8 * j + 2 * t4 + odd, r0 - odd + 16 * half + 8 * h, odd ? got : v[2 * h], odd ? v[2 * h + 1] : got);
+            finish(8 * j + tok0, row0 + 8 * h, odd ? got : v[2 * h], odd ? v[2 * h + 1] : got, j ? beside(8 * j + tok0, row0 + 8 * h) : early[h]);
           }
         }
       continue;
@@ -394,20 +402,29 @@ __global__ void __launch_bounds__(kRThreads, 2) k_ragged(const __grid_constant__
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             sums[(half * NT + 8 * j + 2 * t4 + (i & 1)) * kTileRows + r0 + 16 * m + 8 * (i >> 1)] = acc[m][j][i];
+    const int pairs = t.n * (kTileRows / 2), i0 = tid + split * kRCons * 32;
+    Beside next = beside(i0 / (kTileRows / 2), 2 * (i0 % (kTileRows / 2)));  // under way while the splits meet
     cluster_sync();
-    const int pairs = t.n * (kTileRows / 2);
-    for (int i = tid + split * kRCons * 32; i < pairs && !dead; i += S * kRCons * 32) {
+    for (int i = i0; i < pairs && !dead; i += S * kRCons * 32) {
       const int tok = i / (kTileRows / 2), r = 2 * (i % (kTileRows / 2));
-      float v0 = 0.f, v1 = 0.f;
-      for (int s = 0; s < S; ++s) {
+      float2 v[kRMaxSplit][2];  // every split's loads are in flight together
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float2 v = ld_cluster_f32x2(map_to_rank(smem_u32(sums + (h * NT + tok) * kTileRows + r), s));
-          v0 += v.x;
-          v1 += v.y;
-        }
-      }
-      finish(tok, r, v0, v1);
+      for (int s = 0; s < kRMaxSplit; ++s)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (s < S) v[s][h] = ld_cluster_f32x2(map_to_rank(smem_u32(sums + (h * NT + tok) * kTileRows + r), s));
+      float v0 = 0.f, v1 = 0.f;
+#pragma unroll
+      for (int s = 0; s < kRMaxSplit; ++s)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (s < S) {
+            v0 += v[s][h].x;
+            v1 += v[s][h].y;
+          }
+      finish(tok, r, v0, v1, next);
+      const int in = i + S * kRCons * 32;
+      if (in < pairs) next = beside(in / (kTileRows / 2), 2 * (in % (kTileRows / 2)));
     }
     break;  // (a cluster takes one unit)
   }
