@@ -222,7 +222,7 @@ struct SetTable {
 template <int MODE, bool PAIR>
 __device__ __forceinline__ PTile walk_tile(const PrefillParams& p, int tile, int& set, const SetTable& tab) {
   if constexpr (MODE != kSets) return tile_of<PAIR>(p, tile);
-  while (set + 1 < p.call.sets && tile >= tab.first[set + 1]) ++set;
+  set = set_of(tile, set, tab.first, p.call.sets);
   const int2 b = tab.bounds[set];
   const int n = b.y - b.x, tt = (n + p.tn - 1) / p.tn, per = mma_tokens<PAIR>((n + tt - 1) / tt);
   const int at = tile - tab.first[set];
@@ -373,12 +373,13 @@ __global__ void __launch_bounds__(prefill_warps(MODE) * 32, 1) k_prefill(const _
     tab.bounds = bounds;
     tab.first = first;
     pdl_wait();
+    for (int e = tid; e < p.call.sets; e += prefill_warps(MODE) * 32) bounds[e] = set_slots(p.call.offsets, e, p.call.slots);
+    __syncthreads();
     if (warp == 0) {
       int run = 0;
       for (int e0 = 0; e0 < p.call.sets; e0 += 32) {
         const int e = e0 + lane;
-        int2 b = make_int2(0, 0);
-        if (e < p.call.sets) bounds[e] = b = set_slots(p.call.offsets, e, p.call.slots);
+        const int2 b = e < p.call.sets ? bounds[e] : make_int2(0, 0);
         const int mine = (b.y - b.x + p.tn - 1) / p.tn * p.pairs;
         int upto = mine;
 #pragma unroll

@@ -63,7 +63,7 @@ struct Unit {
 };
 template <int NT>
 __device__ __forceinline__ Unit unit_of(int u, int& e, const int* first, const int2* bounds, int sets) {
-  while (e + 1 < sets && u >= first[e + 1]) ++e;
+  e = set_of(u, e, first, sets);
   const int n = bounds[e].y - bounds[e].x, chunks = (n + NT - 1) / NT, at = u - first[e];
   Unit t;
   t.e = e;
@@ -167,16 +167,19 @@ __global__ void __launch_bounds__(kRThreads, 2) k_ragged(const __grid_constant__
   }
   pdl_launch_dependents();
   if (c.offsets) pdl_wait();  // offsets, and with them everything else, come from the kernels in front
+  if (c.offsets) {
+    for (int e = tid; e < c.sets; e += kRThreads) bounds[e] = set_slots(c.offsets, e, c.slots);
+    __syncthreads();
+  } else if (tid == 0) {
+    bounds[0] = make_int2(0, c.slots);
+  }
   if (warp == 0) {
+    __syncwarp();
     // units of every set: ceil(tokens / NT) chunks of each row tile
     int run = 0;
     for (int e0 = 0; e0 < c.sets; e0 += 32) {
       const int e = e0 + lane;
-      int2 b = make_int2(0, 0);
-      if (e < c.sets) {
-        b = c.offsets ? set_slots(c.offsets, e, c.slots) : make_int2(0, c.slots);
-        bounds[e] = b;
-      }
+      const int2 b = e < c.sets ? bounds[e] : make_int2(0, 0);
       const int mine = (b.y - b.x + NT - 1) / NT * p.row_tiles;
       int upto = mine;
 #pragma unroll

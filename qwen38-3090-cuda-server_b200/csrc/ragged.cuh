@@ -70,6 +70,19 @@ __device__ __forceinline__ int2 set_slots(const int32_t* offsets, int e, int slo
   const int lo = min(max(__ldcg(offsets + e), 0), slots);
   return make_int2(lo, min(max(__ldcg(offsets + e + 1), lo), slots));
 }
+// The set of unit u, from set e on: the last whose first unit is not behind u. By halves, since every step waits for
+// shared memory and most sets may be empty: one token, 8 of 256 experts of 2048 x 1024, 16.8 -> 9.4 us.
+__device__ __forceinline__ int set_of(int u, int e, const int* first, int sets) {
+  if (u < first[e + 1]) return e;
+  for (int last = sets - 1; e < last;) {
+    const int mid = (e + last + 1) >> 1;
+    if (first[mid] <= u)
+      e = mid;
+    else
+      last = mid - 1;
+  }
+  return e;
+}
 #endif
 
 inline bool ranges_apart(const void* a, size_t an, const void* b, size_t bn) {
