@@ -3,6 +3,7 @@
 #include <atomic>
 #include <climits>
 #include <cfloat>
+#include <type_traits>
 
 #include "ragged.cuh"
 
@@ -11,14 +12,20 @@ namespace {
 
 constexpr int kRouteWarps = 32;    // tokens of a block: one warp each, one bit each in the blocks' expert masks
 constexpr int kRouteMaxK = 16;
+constexpr int kRouteFewWarps = 8;  // tokens of a block while that spreads them over more SMs
+constexpr int kRouteFewRows = 256, kRouteFewWords = 8000;  // blocks, and words of their counts, up to which every block adds them up itself
 constexpr int kCombineThreads = 128, kCombineCtas = 8;  // and CTAs per SM
 
 struct RouteParams {
   int32_t *ids, *offsets, *slots, *rows, *counts;
   float* weights;
   const void* logits;
-  int f32, T, E, k, renormalize, blocks;
+  int f32, T, E, k, renormalize;
+  int per, blocks;  // tokens of a block of k_route, and its blocks
+  int few;          // every block adds up the counts itself
 };
+// Counts of a block's tokens per expert, if few: bytes (at most 32), four experts a word. Else words.
+__device__ __forceinline__ int count_words(int E) { return (E + 3) / 4; }
 
 // fp32 as an unsigned key of the same order; -inf and NaN become 0 (never picked), +inf the largest finite value
 __device__ __forceinline__ uint32_t order_key(float v) {
@@ -52,13 +59,14 @@ __device__ __forceinline__ void scan_experts(int* totals, int E, int lane) {
 // With one block the slots follow at once; otherwise the block's counts go out and k_route_scan and k_route_slots finish.
 // Bound by its launches and their dependences: one token of 64 experts 6.3 us as an eager call (5.3 of them the host's; 3.2 in a graph), 4096 tokens of 256
 // experts 16.5 us in three launches, where the logits take 0.7 at HBM's rate. Counts added up by one CTA 28 us, by every block for itself 21.9.
-template <int EPL>
-__global__ void __launch_bounds__(kRouteWarps * 32) k_route(const RouteParams p) {
+template <int EPL, int PER>
+__global__ void __launch_bounds__(PER * 32) k_route(const RouteParams p) {
   __shared__ uint32_t masks[kMaxSets];
   __shared__ int offs[kMaxSets + 1];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int t = blockIdx.x * kRouteWarps + warp;
-  for (int e = tid; e < p.E; e += kRouteWarps * 32) masks[e] = 0;
+  const int t = blockIdx.x * PER + warp;
+  constexpr int threads = PER * 32;
+  for (int e = tid; e < 4 * count_words(p.E); e += threads) masks[e] = 0;
   __syncthreads();
   pdl_launch_dependents();
   pdl_wait();
@@ -130,15 +138,21 @@ __global__ void __launch_bounds__(kRouteWarps * 32) k_route(const RouteParams p)
     }
   }
   __syncthreads();
-  if (p.blocks > 1) {
-    for (int e = tid; e < p.E; e += kRouteWarps * 32) p.counts[static_cast<size_t>(blockIdx.x) * p.E + e] = __popc(masks[e]);
+  if (p.few) {
+    const int w = tid, words = count_words(p.E);
+    if (w < words)
+      p.counts[blockIdx.x * words + w] = __popc(masks[4 * w]) | __popc(masks[4 * w + 1]) << 8 | __popc(masks[4 * w + 2]) << 16 | __popc(masks[4 * w + 3]) << 24;
     return;
   }
-  for (int e = tid; e < p.E; e += kRouteWarps * 32) offs[e] = __popc(masks[e]);
+  if (p.blocks > 1) {
+    for (int e = tid; e < p.E; e += threads) p.counts[static_cast<size_t>(blockIdx.x) * p.E + e] = __popc(masks[e]);
+    return;
+  }
+  for (int e = tid; e < p.E; e += threads) offs[e] = __popc(masks[e]);
   __syncthreads();
   if (warp == 0) scan_experts(offs, p.E, lane);
   __syncthreads();
-  for (int e = tid; e <= p.E; e += kRouteWarps * 32) p.offsets[e] = offs[e];
+  for (int e = tid; e <= p.E; e += threads) p.offsets[e] = offs[e];
   if (my_id >= 0) {
     const int slot = offs[my_id] + __popc(masks[my_id] & ((1u << warp) - 1u));
     p.slots[static_cast<size_t>(t) * p.k + lane] = slot;
@@ -174,7 +188,9 @@ __global__ void __launch_bounds__(kRouteWarps * 32) k_route_scan(const RoutePara
   if (warp == kRouteWarps - 1) column[static_cast<size_t>(p.blocks) * p.E] = run;
 }
 
-// Slots of a block's picks: first slot of the expert, picks of earlier blocks, earlier tokens of the block.
+// Slots of a block's picks: first slot of the expert, picks of earlier blocks, earlier tokens of the block. With few blocks it adds up
+// their counts itself (whole numbers, in any order): a thread takes a word of four experts of some of the blocks and sums the bytes in
+// halves of a word, at most 8192.
 __global__ void __launch_bounds__(kRouteWarps * 32) k_route_slots(const RouteParams p) {
   __shared__ uint32_t masks[kMaxSets];
   __shared__ int offs[kMaxSets + 1], before[kMaxSets];
@@ -186,9 +202,36 @@ __global__ void __launch_bounds__(kRouteWarps * 32) k_route_slots(const RoutePar
   pdl_wait();
   const int id = t < p.T && lane < p.k ? __ldcg(p.ids + static_cast<size_t>(t) * p.k + lane) : -1;
   if (id >= 0) atomicOr(&masks[id], 1u << warp);
-  for (int e = tid; e < p.E; e += kRouteWarps * 32) {
-    offs[e] = __ldcg(p.counts + static_cast<size_t>(p.blocks) * p.E + e);
-    before[e] = __ldcg(p.counts + static_cast<size_t>(blockIdx.x) * p.E + e);
+  if (p.few) {
+    const int mine_end = blockIdx.x * (kRouteWarps / p.per);  // (k_route's blocks may have fewer tokens)
+    const int words = count_words(p.E), w = tid % words, step = kRouteWarps * 32 / words, first = tid / words;
+    const bool takes = first < step && first < p.blocks;
+    uint32_t all[2] = {}, mine[2] = {};
+    if (takes)
+#pragma unroll 8
+      for (int b = first; b < p.blocks; b += step) {
+        const uint32_t v = __ldcg(reinterpret_cast<const uint32_t*>(p.counts) + b * words + w), even = v & 0x00FF00FFu, odd = (v >> 8) & 0x00FF00FFu;
+        all[0] += even;
+        all[1] += odd;
+        if (b < mine_end) {
+          mine[0] += even;
+          mine[1] += odd;
+        }
+      }
+    for (int i = tid; i < 4 * words; i += kRouteWarps * 32) offs[i] = before[i] = 0;
+    __syncthreads();
+    if (takes)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int shift = i & 2 ? 16 : 0;
+        atomicAdd(&offs[4 * w + i], static_cast<int>(all[i & 1] >> shift & 0xFFFFu));
+        atomicAdd(&before[4 * w + i], static_cast<int>(mine[i & 1] >> shift & 0xFFFFu));
+      }
+  } else {
+    for (int e = tid; e < p.E; e += kRouteWarps * 32) {
+      offs[e] = __ldcg(p.counts + static_cast<size_t>(p.blocks) * p.E + e);
+      before[e] = __ldcg(p.counts + static_cast<size_t>(blockIdx.x) * p.E + e);
+    }
   }
   __syncthreads();
   if (warp == 0) scan_experts(offs, p.E, lane);
@@ -358,6 +401,8 @@ int w4a16_route(int32_t* ids, float* weights, int32_t* offsets, int32_t* slots, 
   const int blocks = route_blocks(T);
   if (blocks > 1 && (workspace == nullptr || workspace_bytes < w4a16_route_workspace(T, num_experts)))
     return fail(W4A16_ESCRATCH, "route: workspace of %zu bytes for %d tokens, %zu needed", workspace_bytes, T, w4a16_route_workspace(T, num_experts));
+  const DeviceInfo* di = device_info();
+  if (!di) return W4A16_ECUDA;
   RouteParams p = {};
   p.ids = ids;
   p.weights = weights;
@@ -371,18 +416,31 @@ int w4a16_route(int32_t* ids, float* weights, int32_t* offsets, int32_t* slots, 
   p.E = num_experts;
   p.k = top_k;
   p.renormalize = renormalize != 0;
-  p.blocks = blocks;
-  const dim3 grid(blocks > 0 ? blocks : 1);  // (no tokens: the offsets are still written)
+  // A block of 32 tokens keeps one SM busy for microseconds (512 experts: 8): tokens that would leave SMs idle go eight to a block, as long
+  // as their counts fit the workspace. Counts of few blocks are added up by every block of k_route_slots, of more by a kernel in between.
+  // us in a graph, blocks of 32 and the kernel in between / this: 64 experts, 33 tokens 7.0 / 4.7, 1000 8.1 / 6.7; 256: 10.2 / 7.1,
+  // 12.0 / 11.6; 512: 14.3 / 9.9, 18 / 15.7.
+  // Adding up 16384 words (512 experts, 4096 tokens) 23.6, the kernel in between 22.2.
+  const long long row_words = (num_experts + 3) / 4, narrow = (static_cast<long long>(T) + kRouteFewWarps - 1) / kRouteFewWarps;
+  const bool spread = blocks > 1 && T <= kRouteFewWarps * di->sms && narrow * row_words <= kRouteFewWords &&
+                      narrow * row_words <= (blocks + 1LL) * num_experts;
+  p.per = spread ? kRouteFewWarps : kRouteWarps;
+  p.blocks = spread ? static_cast<int>(narrow) : blocks;
+  p.few = blocks > 1 && (spread || (blocks <= kRouteFewRows && blocks * row_words <= kRouteFewWords));
+  const dim3 grid(p.blocks > 0 ? p.blocks : 1);  // (no tokens: the offsets are still written)
   const int per_lane = (num_experts + 31) / 32;
-  int rc;
-  if (per_lane <= 2) rc = enqueue(k_route<2>, grid, kRouteWarps * 32, p, stream, "route");
-  else if (per_lane <= 4) rc = enqueue(k_route<4>, grid, kRouteWarps * 32, p, stream, "route");
-  else if (per_lane <= 8) rc = enqueue(k_route<8>, grid, kRouteWarps * 32, p, stream, "route");
-  else rc = enqueue(k_route<16>, grid, kRouteWarps * 32, p, stream, "route");
+  auto picks = [&](auto per) {
+    constexpr int PER = decltype(per)::value;
+    if (per_lane <= 2) return enqueue(k_route<2, PER>, grid, PER * 32, p, stream, "route");
+    if (per_lane <= 4) return enqueue(k_route<4, PER>, grid, PER * 32, p, stream, "route");
+    if (per_lane <= 8) return enqueue(k_route<8, PER>, grid, PER * 32, p, stream, "route");
+    return enqueue(k_route<16, PER>, grid, PER * 32, p, stream, "route");
+  };
+  int rc = spread ? picks(std::integral_constant<int, kRouteFewWarps>()) : picks(std::integral_constant<int, kRouteWarps>());
   if (rc != W4A16_OK || blocks <= 1) return rc;
-  rc = enqueue(k_route_scan, dim3((num_experts + 31) / 32), kRouteWarps * 32, p, stream, "route");
+  if (!p.few) rc = enqueue(k_route_scan, dim3((num_experts + 31) / 32), kRouteWarps * 32, p, stream, "route");
   if (rc != W4A16_OK) return rc;
-  return enqueue(k_route_slots, grid, kRouteWarps * 32, p, stream, "route");
+  return enqueue(k_route_slots, dim3(blocks), kRouteWarps * 32, p, stream, "route");
 }
 
 int w4a16_experts_combine(uint16_t* y, const uint16_t* parts, int parts_rows, const int32_t* slots, const float* weights,
