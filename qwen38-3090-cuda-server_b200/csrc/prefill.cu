@@ -375,23 +375,8 @@ __global__ void __launch_bounds__(prefill_warps(MODE) * 32, 1) k_prefill(const _
     pdl_wait();
     for (int e = tid; e < p.call.sets; e += prefill_warps(MODE) * 32) bounds[e] = set_slots(p.call.offsets, e, p.call.slots);
     __syncthreads();
-    if (warp == 0) {
-      int run = 0;
-      for (int e0 = 0; e0 < p.call.sets; e0 += 32) {
-        const int e = e0 + lane;
-        const int2 b = e < p.call.sets ? bounds[e] : make_int2(0, 0);
-        const int mine = (b.y - b.x + p.tn - 1) / p.tn * p.pairs;
-        int upto = mine;
-#pragma unroll
-        for (int d = 1; d < 32; d *= 2) {
-          const int v = __shfl_up_sync(0xffffffffu, upto, d);
-          if (lane >= d) upto += v;
-        }
-        if (e < p.call.sets) first[e] = run + upto - mine;
-        run += __shfl_sync(0xffffffffu, upto, 31);
-      }
-      if (lane == 0) first[p.call.sets] = run;
-    }
+    if (warp == 0)
+      prefix_sums(first, p.call.sets, lane, [&](int e) { return (bounds[e].y - bounds[e].x + p.tn - 1) / p.tn * p.pairs; });
     __syncthreads();
     tiles = first[p.call.sets];
   }

@@ -167,30 +167,15 @@ __global__ void __launch_bounds__(kRThreads, 2) k_ragged(const __grid_constant__
   }
   pdl_launch_dependents();
   if (c.offsets) pdl_wait();  // offsets, and with them everything else, come from the kernels in front
+  // units of every set: ceil(tokens / NT) chunks of each row tile
   if (c.offsets) {
     for (int e = tid; e < c.sets; e += kRThreads) bounds[e] = set_slots(c.offsets, e, c.slots);
     __syncthreads();
+    if (warp == 0) prefix_sums(first, c.sets, lane, [&](int e) { return (bounds[e].y - bounds[e].x + NT - 1) / NT * p.row_tiles; });
   } else if (tid == 0) {
     bounds[0] = make_int2(0, c.slots);
-  }
-  if (warp == 0) {
-    __syncwarp();
-    // units of every set: ceil(tokens / NT) chunks of each row tile
-    int run = 0;
-    for (int e0 = 0; e0 < c.sets; e0 += 32) {
-      const int e = e0 + lane;
-      const int2 b = e < c.sets ? bounds[e] : make_int2(0, 0);
-      const int mine = (b.y - b.x + NT - 1) / NT * p.row_tiles;
-      int upto = mine;
-#pragma unroll
-      for (int d = 1; d < 32; d *= 2) {
-        const int v = __shfl_up_sync(0xffffffffu, upto, d);
-        if (lane >= d) upto += v;
-      }
-      if (e < c.sets) first[e] = run + upto - mine;
-      run += __shfl_sync(0xffffffffu, upto, 31);
-    }
-    if (lane == 0) first[c.sets] = run;
+    first[0] = 0;
+    first[1] = (c.slots + NT - 1) / NT * p.row_tiles;
   }
   __syncthreads();
   const int units = first[c.sets];

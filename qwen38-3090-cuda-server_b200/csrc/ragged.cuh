@@ -70,6 +70,27 @@ __device__ __forceinline__ int2 set_slots(const int32_t* offsets, int e, int slo
   const int lo = min(max(__ldcg(offsets + e), 0), slots);
   return make_int2(lo, min(max(__ldcg(offsets + e + 1), lo), slots));
 }
+// Prefix sums of value(0 .. n - 1) into first[0 .. n], the sum in first[n], by one whole warp: a lane takes neighbours. (32 at a time with a
+// carry, 256 experts at one token 12.1 us instead of 11.7.)
+template <class F>
+__device__ __forceinline__ void prefix_sums(int* first, int n, int lane, F value) {
+  const int per = (n + 31) / 32, i0 = min(lane * per, n), i1 = min(i0 + per, n);
+  int mine = 0;
+  for (int i = i0; i < i1; ++i) mine += value(i);
+  int upto = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const int v = __shfl_up_sync(0xffffffffu, upto, d);
+    if (lane >= d) upto += v;
+  }
+  int run = upto - mine;
+  for (int i = i0; i < i1; ++i) {
+    const int v = value(i);
+    first[i] = run;
+    run += v;
+  }
+  if (lane == 31) first[n] = run;
+}
 // The set of unit u, from set e on: the last whose first unit is not behind u. By halves, since every step waits for
 // shared memory and most sets may be empty: one token, 8 of 256 experts of 2048 x 1024, 16.8 -> 9.4 us.
 __device__ __forceinline__ int set_of(int u, int e, const int* first, int sets) {

@@ -266,6 +266,12 @@ def test_route_sizes(pkg, E, k, renormalize, T):
     _check_route(pkg, logits.to(torch.bfloat16), k, renormalize)
 
 
+@pytest.mark.parametrize("T,E,k", [(1184, 64, 8), (1185, 64, 8), (4000, 12, 3), (8192, 20, 2), (8193, 20, 2), (250, 512, 16), (513, 512, 4), (300, 5, 5), (40, 1, 1)])
+def test_route_borders_of_its_launches(pkg, T, E, k):
+    """Eight tokens to a block or 32, counts added up by every block or in between."""
+    _check_route(pkg, torch.randn((T, E), generator=torch.Generator().manual_seed(T)).cuda(), k)
+
+
 def test_route_many_tokens(pkg):
     _check_route(pkg, torch.randn((9000, 40), generator=torch.Generator().manual_seed(1)).cuda().to(torch.bfloat16), 4)
 
