@@ -16,7 +16,7 @@
 //
 // What bounds it: the expansion's instructions. Two CTAs of an SM take some 500 cycles for a weight block where HBM allows 370: 1460
 // warp instructions at M = 8, of which LOP3, shifts and packed bf16 arithmetic issue at half a scheduler's rate (measured by themselves: 345 cycles without
-// the mma.sync, 408 with). 34816 x 5120 at M = 8 25.1 us (3.7 TB/s), 64 experts 5120 x 1024 at 4.1 slots each 52.8 (3.3 TB/s).
+// the mma.sync, 408 with). 34816 x 5120 at M = 8 24.8 us (3.7 TB/s), 64 experts 5120 x 1024 at 4.1 slots each 52 (3.4 TB/s).
 // Tried beside it, the same or slower: 16 rows x 128 k per warp, three CTAs per SM, loads a step ahead, more accumulators, and A in tensor memory for
 // tcgen05.mma with two CTAs per SM (28.5 us at M = 1 against 25).
 #include <climits>
@@ -536,7 +536,7 @@ int run_ragged(RaggedCall& c, const char* who, cudaStream_t st) {
   p.status = di->status;
   // More than a few tokens per set: whole tiles on tcgen05, whose time hardly depends on their number up to 128 (here every eight
   // tokens cost 64 mma.sync per weight block, beside 1040 instructions for its expansion), but which cost more at both ends, so that
-  // short rows of weights stay here longer. us, here / there: 16384 x 5120 at M = 8 15.5 / 17.1, at 16 19.0 / 17.3; 2048 x 5120 in 64 sets of 4.1 in
+  // short rows of weights stay here longer. us, here / there: 34816 x 5120 at M = 8 24.8 / 27.9, at 16 30.0 / 28.3; 16384 x 5120 at 16 20.1 / 16.3; 2048 x 5120 in 64 sets of 4.1 in
   // the mean 87.6 / 97.2, of 5 102 / 97, of 6.5 107 / 99; 2048 x 2048 in 256 of 5.6 145 / 149, of 6.5 152 / 151, of 7.5 163 / 156; 5120 x 1024 in 64
   // of 5 56.5 / 61.1, of 6.5 62.6 / 62.8, of 8.5 66.6 / 63.5.
   if (c.offsets ? 2LL * c.slots > (c.G >= 32 ? 9LL : 13LL) * c.sets : c.slots > 8) return launch_prefill_ragged(c, st);

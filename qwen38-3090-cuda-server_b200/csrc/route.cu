@@ -53,11 +53,11 @@ __device__ __forceinline__ void scan_experts(int* totals, int E, int lane) {
   if (lane == 0) totals[E] = run;
 }
 
-// Picks of a block of 32 tokens: a warp per token holds its logits in registers, EPL per lane (expert 32 i + lane). k times the
+// Picks of a block of PER tokens: a warp per token holds its logits in registers, EPL per lane (expert 32 i + lane). k times the
 // largest key over the warp, then the lowest index that has it. Within a block the tokens that picked an expert are the bits of a
 // word, so that a pick's place among them is a population count: sorted by expert and token without sorting.
 // With one block the slots follow at once; otherwise the block's counts go out and k_route_scan and k_route_slots finish.
-// Bound by its launches and their dependences: one token of 64 experts 6.3 us as an eager call (5.3 of them the host's; 3.2 in a graph), 4096 tokens of 256
+// Bound by its launches and their dependences: one token of 64 experts 5.7 us as an eager call, nearly all the host's (3.2 in a graph), 4096 tokens of 256
 // experts 16.5 us in three launches, where the logits take 0.7 at HBM's rate. Counts added up by one CTA 28 us, by every block for itself 21.9.
 template <int EPL, int PER>
 __global__ void __launch_bounds__(PER * 32) k_route(const RouteParams p) {
