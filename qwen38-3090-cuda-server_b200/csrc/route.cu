@@ -14,7 +14,7 @@ constexpr int kRouteWarps = 32;    // tokens of a block: one warp each, one bit 
 constexpr int kRouteMaxK = 16;
 constexpr int kRouteFewWarps = 8;  // tokens of a block while that spreads them over more SMs
 constexpr int kRouteFewRows = 256, kRouteFewWords = 8000;  // blocks, and words of their counts, up to which every block adds them up itself
-constexpr int kCombineThreads = 128, kCombineCtas = 8;  // and CTAs per SM
+constexpr int kCombineThreads = 128, kCombineCtas = 8;  // and CTAs per SM at most
 
 struct RouteParams {
   int32_t *ids, *offsets, *slots, *rows, *counts;
@@ -250,23 +250,13 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool r
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// All but the n latest groups of this thread have landed.
-__device__ __forceinline__ void cp_async_wait_but(int n) {
-  switch (n) {
-    case 2: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
-    case 4: asm volatile("cp.async.wait_group 4;" ::: "memory"); break;
-    default: asm volatile("cp.async.wait_group 7;" ::: "memory");
-  }
-}
-
 struct CombineParams {
   uint16_t* y;
   const uint16_t *parts, *residual;
   const int32_t* slots;
   const float* weights;
-  int parts_rows, k, H;
-  uint32_t strips, items;  // strips of 256 columns, T x strips
-  int depth;               // 3, 5 or 8 items in the ring
+  int parts_rows, T, k, H;
+  uint32_t strips;  // of 256 columns
 };
 
 __device__ __forceinline__ void add_row(float (&s)[8], const uint4& v, float w) {
@@ -278,83 +268,98 @@ __device__ __forceinline__ void add_row(float (&s)[8], const uint4& v, float w) 
   }
 }
 
-// A warp takes 256 columns of a token at a time, eight per lane, its picks' rows by asynchronous copies through a ring of `depth` items in
-// shared memory: a lane copies and reads its own 16 bytes of every row only, so that no barrier is needed, and the bytes in
-// flight take no registers. Empty picks are filled with zeros. Bound by HBM: 4096 tokens of 8 picks x 5120, a tenth empty, 76 us (5.1 TB/s); with the
-// rows in registers (28 warps per SM, one item each) 100.
+// A warp takes 256 columns of a token at a time, eight per lane: the picks' rows and the residual's by asynchronous copies through a ring
+// in shared memory. A lane copies and reads its own 16 bytes of every row only, so that no barrier is needed, and the bytes in
+// flight take no registers. Empty picks are filled with zeros. Bound by HBM: 4096 tokens of 8 picks x 5120, a tenth empty, 62.6 us (6.2 TB/s). On the way: rows in
+// registers 100; a ring of three items 76; the residual in the ring and two items 65 (its load had been waited for where it is added); items counted
+// on instead of four divisions each 66 with two items, 62.6 with four (4 picks x 5120 54.7 -> 39.6, one pick 36.2 -> 24.0).
+template <int DEPTH>  // items of a warp in shared memory
 __global__ void __launch_bounds__(kCombineThreads) k_combine(const CombineParams p) {
   extern __shared__ __align__(16) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t stage = p.k * 512 + kRouteMaxK * 4;  // rows, then the weights
-  const uint32_t ring = smem_u32(smem) + warp * p.depth * stage;
+  const int rows = p.k + (p.residual ? 1 : 0);
+  const uint32_t item_bytes = rows * 512 + kRouteMaxK * 4;  // rows, the residual's among them, then the weights
+  const uint32_t ring = smem_u32(smem) + warp * DEPTH * item_bytes;
   pdl_launch_dependents();
   pdl_wait();
   const uint32_t stride = gridDim.x * (kCombineThreads / 32), first = blockIdx.x * (kCombineThreads / 32) + warp;
-  // lane j's pick j of an item, two steps before the item's copies start
-  auto pick = [&](uint32_t item, int& slot, float& w) {
+  const uint32_t step_t = stride / p.strips, step_s = stride - step_t * p.strips, T = p.T;
+  struct Item {
+    uint32_t t, strip;
+  };
+  auto behind = [&](Item i) {
+    i.t += step_t;
+    i.strip += step_s;
+    if (i.strip >= p.strips) {
+      i.strip -= p.strips;
+      ++i.t;
+    }
+    return i;
+  };
+  // lane j's pick j of an item, one step before the item's copies start
+  int slot;
+  float weight;
+  auto pick = [&](const Item& i) {
     slot = -1;
-    w = 0.f;
-    if (item < p.items && lane < p.k) {
-      const size_t o = static_cast<size_t>(item / p.strips) * p.k + lane;
+    weight = 0.f;
+    if (i.t < T && lane < p.k) {
+      const size_t o = static_cast<size_t>(i.t) * p.k + lane;
       slot = __ldcg(p.slots + o);
-      w = __ldcg(p.weights + o);
-      if (slot >= p.parts_rows) slot = -1;
+      weight = __ldcg(p.weights + o);
     }
   };
-  auto start = [&](uint32_t item, uint32_t to, int slot, float w) {
-    if (item < p.items) {
-      const int col = static_cast<int>(item % p.strips) * 256 + lane * 8;
+  auto start = [&](const Item& i, uint32_t to, int row_of, float w) {
+    if (i.t < T) {
+      const int mine = row_of < p.parts_rows ? row_of : -1;
+      const int col = i.strip * 256 + lane * 8;
       const bool inside = col < p.H;
+      const uint16_t* src = p.parts + (inside ? col : 0);
+      const uint32_t dst = to + lane * 16;
 #pragma unroll 4
       for (int j = 0; j < p.k; ++j) {
-        const int row = __shfl_sync(0xffffffffu, slot, j);
-        const bool real = row >= 0 && inside;
-        cp_async16(to + j * 512 + lane * 16, p.parts + (real ? static_cast<size_t>(row) * p.H + col : 0), real);
+        const int row = __shfl_sync(0xffffffffu, mine, j);
+        cp_async16(dst + j * 512, src + static_cast<size_t>(max(row, 0)) * p.H, row >= 0 && inside);
       }
-      if (lane < p.k) sts32(to + p.k * 512 + lane * 4, __float_as_uint(slot >= 0 ? w : 0.f));
+      if (p.residual) cp_async16(dst + p.k * 512, p.residual + static_cast<size_t>(i.t) * p.H + (inside ? col : 0), inside);
+      if (lane < p.k) sts32(to + rows * 512 + lane * 4, __float_as_uint(mine >= 0 ? w : 0.f));
     }
     cp_async_commit();
   };
-  int slot;
-  float weight;
-  pick(first, slot, weight);
-  uint32_t ahead = first;
-  for (int i = 0; i < p.depth - 1; ++i, ahead += stride) {
-    int next_slot;
-    float next_weight;
-    pick(ahead + stride, next_slot, next_weight);
-    start(ahead, ring + i * stage, slot, weight);
-    slot = next_slot;
-    weight = next_weight;
+  Item item = {first / p.strips, first % p.strips}, ahead = item;
+  pick(item);
+  for (int i = 0; i < DEPTH - 1; ++i) {
+    const int row_of = slot;
+    const float w = weight;
+    const Item now = ahead;
+    ahead = behind(ahead);
+    pick(ahead);
+    start(now, ring + i * item_bytes, row_of, w);
   }
-  int st = 0, st_ahead = p.depth - 1;
-  for (uint32_t item = first; item < p.items; item += stride, ahead += stride) {
-    int next_slot;
-    float next_weight;
-    pick(ahead + stride, next_slot, next_weight);
-    __syncwarp();  // every lane has read the weights that the stage held
-    start(ahead, ring + st_ahead * stage, slot, weight);
-    slot = next_slot;
-    weight = next_weight;
-    cp_async_wait_but(p.depth - 1);
+  int st = 0, st_ahead = DEPTH - 1;
+  for (; item.t < T; item = behind(item)) {
+    const int row_of = slot;
+    const float w = weight;
+    const Item now = ahead;
+    ahead = behind(ahead);
+    pick(ahead);
+    __syncwarp();  // every lane has read the weights that the place held
+    start(now, ring + st_ahead * item_bytes, row_of, w);
+    asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory");
     __syncwarp();
-    const uint32_t t = item / p.strips, at = ring + st * stage;
-    const int col = static_cast<int>(item - t * p.strips) * 256 + lane * 8;
-    const size_t o = static_cast<size_t>(t) * p.H + col;
-    uint4 r = make_uint4(0, 0, 0, 0);
-    if (p.residual && col < p.H) r = *reinterpret_cast<const uint4*>(p.residual + o);
+    const uint32_t at = ring + st * item_bytes;
+    const int col = item.strip * 256 + lane * 8;
     float s[8] = {};
 #pragma unroll 8
-    for (int j = 0; j < p.k; ++j) add_row(s, lds128<0>(at + j * 512 + lane * 16), __uint_as_float(lds32(at + p.k * 512 + j * 4)));
-    if (p.residual) add_row(s, r, 1.f);
+    for (int j = 0; j < p.k; ++j) add_row(s, lds128<0>(at + j * 512 + lane * 16), __uint_as_float(lds32(at + rows * 512 + j * 4)));
+    if (p.residual) add_row(s, lds128<0>(at + p.k * 512 + lane * 16), 1.f);
     if (col < p.H) {
       uint32_t out[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) out[i] = float_to_bf16_bits(s[2 * i]) | (static_cast<uint32_t>(float_to_bf16_bits(s[2 * i + 1])) << 16);
-      *reinterpret_cast<uint4*>(p.y + o) = make_uint4(out[0], out[1], out[2], out[3]);
+      *reinterpret_cast<uint4*>(p.y + static_cast<size_t>(item.t) * p.H + col) = make_uint4(out[0], out[1], out[2], out[3]);
     }
-    if (++st == p.depth) st = 0;
-    if (++st_ahead == p.depth) st_ahead = 0;
+    if (++st == DEPTH) st = 0;
+    if (++st_ahead == DEPTH) st_ahead = 0;
   }
 }
 
@@ -463,19 +468,24 @@ int w4a16_experts_combine(uint16_t* y, const uint16_t* parts, int parts_rows, co
   if (!di) return W4A16_ECUDA;
   const uint32_t strips = (static_cast<uint32_t>(hidden) + 255) / 256;
   W4_REQUIRE(static_cast<unsigned long long>(T) * strips <= INT_MAX, "experts_combine: %d tokens x %d are too many for one call", T, hidden);
-  // some 24 rows of 512 bytes in flight per warp, four CTAs of four warps per SM
-  const int depth = top_k <= 3 ? 8 : top_k <= 5 ? 5 : 3;
-  const CombineParams p = {y, parts, residual, slots, weights, parts_rows, top_k, hidden, strips, static_cast<uint32_t>(T) * strips, depth};
-  const int smem = kCombineThreads / 32 * depth * (top_k * 512 + kRouteMaxK * 4);
+  const CombineParams p = {y, parts, residual, slots, weights, parts_rows, T, top_k, hidden, strips};
+  // Two items in the ring leave room for more warps, four keep more bytes in flight: us, two / four: 4096 tokens, 5120 columns of 4 picks 42.8 / 39.6, of 8
+  // 66.2 / 62.6, 2048 columns of 16 47.1 / 59.6, 4096 of 2 23.1 / 23.6; where a warp has few items: 300 tokens, 8 picks x 5120 7.2 / 7.9, 1024 x 2048 9.1 / 9.7.
+  const uint32_t items = static_cast<uint32_t>(T) * strips;
+  const bool four = top_k > 2 && top_k <= 8 && items >= 128u * di->sms;
+  const int smem = kCombineThreads / 32 * (four ? 4 : 2) * ((top_k + (residual ? 1 : 0)) * 512 + kRouteMaxK * 4);
   static std::atomic<bool> ready[64];
   if (!ready[di->device & 63].load(std::memory_order_acquire)) {
-    W4_CUDA(cudaFuncSetAttribute(k_combine, cudaFuncAttributeMaxDynamicSharedMemorySize, di->smem_optin));
+    W4_CUDA(cudaFuncSetAttribute(k_combine<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, di->smem_optin));
+    W4_CUDA(cudaFuncSetAttribute(k_combine<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, di->smem_optin));
     ready[di->device & 63].store(true, std::memory_order_release);
   }
   const int fit = di->smem_per_sm / (smem + di->smem_reserved);
-  const uint32_t ctas = (p.items + kCombineThreads / 32 - 1) / (kCombineThreads / 32);
+  const uint32_t ctas = (items + kCombineThreads / 32 - 1) / (kCombineThreads / 32);
   const uint32_t most = static_cast<uint32_t>(di->sms) * (fit < kCombineCtas ? fit : kCombineCtas);
-  return enqueue(k_combine, dim3(ctas < most ? ctas : most), kCombineThreads, p, stream, "experts_combine", smem);
+  const dim3 grid(ctas < most ? ctas : most);
+  return four ? enqueue(k_combine<4>, grid, kCombineThreads, p, stream, "experts_combine", smem)
+              : enqueue(k_combine<2>, grid, kCombineThreads, p, stream, "experts_combine", smem);
 }
 
 }  // extern "C"
