@@ -32,8 +32,8 @@
 //
 // What bounds it: long prompts run at the tensor cores' rate under the power cap (256 x 256 x 16 per 128 cycles: 1024
 // cycles per k group; tensor pipe 87 % active over a 4096-token launch), short ones by no single role: a CTA and k group takes
-// 640 to 700 cycles (5120 x 17408 at M = 77: issue slots 52 %, ALU pipe 41 % on average and 52 % on the busiest SM, tensor pipe 43 % of active
-// cycles), where HBM would allow 386.
+// 560 to 640 cycles (5120 x 17408 at M = 77, before rows were stored sixteen registers at a time: issue slots 52 %, ALU pipe 41 % on average and 52 %
+// on the busiest SM, tensor pipe 43 % of active cycles), where HBM would allow 386.
 // In us, weights cold, against one CTA per tile of 128 x 256 with eight dequant warps (by box and temperature: 2 to 10 %):
 //   34816 x 5120, M = 4096: 1264 -> 922 (1583 TFLOP/s); 5120 x 17408, M = 4096: 698 -> 488 (1497)
 //   34816 x 5120, M = 777:   300 -> 195;                5120 x 8192, M = 777:   110 -> 49

@@ -312,7 +312,7 @@ def test_route_no_tokens_and_refusals(pkg):
 
 
 # ------------------------------------------------------------------ combination
-@pytest.mark.parametrize("T,k,H", [(1, 1, 8), (1, 8, 5120), (3, 9, 1032), (70, 2, 16), (513, 8, 2048), (5, 16, 8200)])
+@pytest.mark.parametrize("T,k,H", [(1, 1, 8), (1, 8, 5120), (3, 9, 1032), (70, 2, 16), (513, 8, 2048), (5, 16, 8200), (2500, 5, 2056), (4000, 8, 1288), (9000, 3, 520), (1000, 2, 5120)])
 @pytest.mark.parametrize("residual", [None, "apart", "in place"])
 def test_combine(pkg, T, k, H, residual):
     """fp32 sums of k + 1 terms, each rounding at most 2^-24 of the sum of magnitudes (products by fma), then one to bf16."""
