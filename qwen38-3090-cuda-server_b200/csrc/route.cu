@@ -58,7 +58,7 @@ __device__ __forceinline__ void scan_experts(int* totals, int E, int lane) {
 // word, so that a pick's place among them is a population count: sorted by expert and token without sorting.
 // With one block the slots follow at once; otherwise the block's counts go out and k_route_scan and k_route_slots finish.
 // Bound by its launches and their dependences: one token of 64 experts 5.7 us as an eager call, nearly all the host's (3.2 in a graph), 4096 tokens of 256
-// experts 16.5 us in three launches, where the logits take 0.7 at HBM's rate. Counts added up by one CTA 28 us, by every block for itself 21.9.
+// experts 15.7 us in three launches, where the logits take 0.7 at HBM's rate. Counts added up by one CTA 28 us, by every block for itself 21.9.
 template <int EPL, int PER>
 __global__ void __launch_bounds__(PER * 32) k_route(const RouteParams p) {
   __shared__ uint32_t masks[kMaxSets];
@@ -84,17 +84,31 @@ __global__ void __launch_bounds__(PER * 32) k_route(const RouteParams p) {
     }
     uint32_t my_key = 0, top = 0;
     float all = 0.f;  // sum of exp over every expert
-    uint32_t best = 0;  // the lane's largest key and the first place that has it
-    int place = 0;
+    // The lane's largest key and the first place that has it. With eight keys also the second largest: a lane that is picked goes on with that, and looks
+    // for two more when it is picked again, which few lanes are (256 experts, 4096 tokens 15.9 -> 14.9 us; with two or four keys 3 % slower, with sixteen
+    // 22.3 -> 16.0 at 4096 tokens, but 22.3 -> 24.4 at 8192: its registers leave room for one block per SM).
+    constexpr bool TWO = EPL == 8;
+    uint32_t best = 0, next = 0, gone = 0;  // (TWO: the places picked, where key stays as it is)
+    int place = 0, next_place = 0;
+    bool have_next = TWO;
     auto largest = [&]() {
-      best = key[0];
+      best = next = 0;
       place = 0;
 #pragma unroll
-      for (int i = 1; i < EPL; ++i)
-        if (key[i] > best) {
-          best = key[i];
+      for (int i = 0; i < EPL; ++i) {
+        const uint32_t v = TWO && (gone >> i & 1u) ? 0u : key[i];
+        if (v > best) {
+          if constexpr (TWO) {
+            next = best;
+            next_place = place;
+          }
+          best = v;
           place = i;
+        } else if (TWO && v > next) {
+          next = v;
+          next_place = i;
         }
+      }
     };
     largest();
     for (int j = 0; j < p.k; ++j) {
@@ -112,10 +126,20 @@ __global__ void __launch_bounds__(PER * 32) k_route(const RouteParams p) {
       }
       const int at = __reduce_min_sync(0xffffffffu, best == most ? 32 * place + lane : INT_MAX);
       if ((at & 31) == lane) {  // only this lane looks for its next largest
+        if constexpr (TWO) {
+          gone |= 1u << place;
+        } else {
 #pragma unroll
-        for (int i = 0; i < EPL; ++i)
-          if (i == place) key[i] = 0;
-        largest();
+          for (int i = 0; i < EPL; ++i)
+            if (i == place) key[i] = 0;
+        }
+        if (TWO && have_next) {
+          best = next;
+          place = next_place;
+        } else {
+          largest();
+        }
+        have_next = TWO && !have_next;
       }
       if (lane == j) {
         my_id = at;
