@@ -27,13 +27,14 @@ struct RouteParams {
 // Counts of a block's tokens per expert, if few: bytes (at most 32), four experts a word. Else words.
 __device__ __forceinline__ int count_words(int E) { return (E + 3) / 4; }
 
-// fp32 as an unsigned key of the same order; -inf and NaN become 0 (never picked), +inf the largest finite value
+// fp32 as an unsigned key of the same order; -inf and NaN become 0 (never picked), +inf the largest finite value. Negative numbers are
+// negated as integers, not complemented: -0 so gets the key of +0, and the two are a tie.
 __device__ __forceinline__ uint32_t order_key(float v) {
   if (!(v > -INFINITY)) return 0;
   const uint32_t u = __float_as_uint(fminf(v, FLT_MAX));
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+  return u & 0x80000000u ? 0u - u : u | 0x80000000u;
 }
-__device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k); }
+__device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : 0u - k); }
 
 // Exclusive prefix sum of one int per expert (in place over totals[0, E)), the sum in totals[E]. Called by one whole warp.
 __device__ __forceinline__ void scan_experts(int* totals, int E, int lane) {
