@@ -459,20 +459,38 @@ def experts_linear(y, w: Experts, x, offsets, x_rows=None, bias=None, activation
 
 class Route:
     """What `route` writes, for up to max_tokens tokens: ids, weights, slots [max_tokens, top_k], offsets [experts + 1],
-    rows [max_tokens * top_k], and its workspace. One call in flight per Route."""
+    rows [max_tokens * top_k], and its workspace. One call in flight per Route. The tables stay where they are, as captured calls write
+    there too: their contents may be changed (r.weights *= 2), another tensor in their place is refused."""
+
+    _FIXED = frozenset(("max_tokens", "num_experts", "top_k", "ids", "weights", "offsets", "slots", "rows"))
 
     def __init__(self, max_tokens: int, num_experts: int, top_k: int):
         import torch
+        if max_tokens < 0 or num_experts < 1 or top_k < 1:
+            raise W4A16Error(-1, f"route: room for {max_tokens} tokens, {top_k} of {num_experts} experts")
         self.max_tokens, self.num_experts, self.top_k = max_tokens, num_experts, top_k
-
-        def make(*shape, dtype=torch.int32):
-            return torch.zeros(shape, dtype=dtype, device="cuda")
-
-        self.ids, self.slots, self.weights = make(max_tokens, top_k), make(max_tokens, top_k), make(max_tokens, top_k, dtype=torch.float32)
-        self.offsets, self.rows = make(num_experts + 1), make(max_tokens * top_k)
+        # One piece of memory that belongs to this object, whatever happens to the tensors that show its parts.
+        sizes = [max_tokens * top_k, max_tokens * top_k, num_experts + 1, max_tokens * top_k, max_tokens * top_k]
+        starts = [0]
+        for n in sizes:
+            starts.append(starts[-1] + (n + 3) // 4 * 4)
+        self._memory = torch.zeros(starts[-1], dtype=torch.int32, device="cuda")
+        self._starts, self._at, self._pointers = starts[:-1], None, []
+        ids, weights, offsets, slots, rows = (self._memory[at:at + n] for at, n in zip(starts, sizes))
+        self.ids, self.slots = ids.view(max_tokens, top_k), slots.view(max_tokens, top_k)
+        self.weights = weights.view(torch.float32).view(max_tokens, top_k)
+        self.offsets, self.rows = offsets, rows
         self.workspace_bytes = lib().w4a16_route_workspace(max_tokens, num_experts)
-        self.workspace = make(self.workspace_bytes // 4)
-        self.pointers = [t.data_ptr() for t in (self.ids, self.weights, self.offsets, self.slots, self.rows)]
+        self.workspace = torch.zeros(self.workspace_bytes // 4, dtype=torch.int32, device="cuda")
+
+    def _find(self, at: int):
+        """The addresses of ids, weights, offsets, slots and rows in the memory, which now is at `at`."""
+        self._at, self._pointers = at, [at + 4 * start for start in self._starts]
+
+    def __setattr__(self, name, value):
+        if name in self._FIXED and getattr(self, name, value) is not value:
+            raise W4A16Error(-1, f"route: {name} stays in its place; change its contents (copy_, mul_), or hand your own tensor to the call that reads it")
+        object.__setattr__(self, name, value)
 
 
 def route_alloc(max_tokens: int, num_experts: int, top_k: int) -> Route:
@@ -488,7 +506,10 @@ def route(r: Route, logits, renormalize: bool = True, stream=None):
     dev, f32 = _device(), logits.dtype is _F32
     _want("route: logits", logits, _F32 if f32 else _BF16, T * r.num_experts, dev)
     _want("route: workspace", r.workspace, _I32, r.workspace_bytes // 4, dev)
-    check(lib().w4a16_route(*r.pointers, logits.data_ptr(), 1 if f32 else 0, T, r.num_experts, r.top_k, 1 if renormalize else 0,
+    memory = r._memory.data_ptr()
+    if memory != r._at:
+        r._find(memory)
+    check(lib().w4a16_route(*r._pointers, logits.data_ptr(), 1 if f32 else 0, T, r.num_experts, r.top_k, 1 if renormalize else 0,
                             r.workspace.data_ptr(), r.workspace_bytes, _stream_of(stream, dev)))
 
 
