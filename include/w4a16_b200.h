@@ -252,8 +252,8 @@ int w4a16_experts_view(const w4a16_experts_t* w, int expert, w4a16_weights_t* vi
  *   y       bf16 [slots][out_f] (SWIGLU: [slots][out_f / 2]); rows behind offsets[num_experts] stay as they were
  *   x       bf16 [x_tokens][in_f]; x_rows int32 [slots], each in [0, x_tokens)
  *   offsets int32 [num_experts + 1], ascending from 0, the last at most `slots`, as w4a16_route writes them. Both tables are read on the
- *           device; bounds and rows outside these ranges are clamped into them, so that no call leaves its buffers, but what
- *           it then writes into y is not specified.
+ *           device; bounds and rows outside these ranges are clamped into them, and a bound below one in front of it counts as
+ *           that one, so that no call leaves its buffers, waits or writes a slot twice; what y then holds is not specified.
  *   bias    bf16 [num_experts][out_f] or NULL; activation, precision and alignment as in w4a16_linear_epilogue.
  * Experts without slots cost nothing. One launch. y must not overlap x, bias, offsets or x_rows. */
 int w4a16_experts_linear(uint16_t* y, const w4a16_experts_t* w, const uint16_t* x, int x_tokens, const int32_t* x_rows,

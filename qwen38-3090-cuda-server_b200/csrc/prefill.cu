@@ -373,8 +373,7 @@ __global__ void __launch_bounds__(prefill_warps(MODE) * 32, 1) k_prefill(const _
     tab.bounds = bounds;
     tab.first = first;
     pdl_wait();
-    for (int e = tid; e < p.call.sets; e += prefill_warps(MODE) * 32) bounds[e] = set_slots(p.call.offsets, e, p.call.slots);
-    __syncthreads();
+    load_bounds<prefill_warps(MODE) * 32>(bounds, p.call.offsets, p.call.sets, p.call.slots, tid);
     if (warp == 0)
       prefix_sums(first, p.call.sets, lane, [&](int e) { return (bounds[e].y - bounds[e].x + p.tn - 1) / p.tn * p.pairs; });
     __syncthreads();

@@ -169,8 +169,7 @@ __global__ void __launch_bounds__(kRThreads, 2) k_ragged(const __grid_constant__
   if (c.offsets) pdl_wait();  // offsets, and with them everything else, come from the kernels in front
   // units of every set: ceil(tokens / NT) chunks of each row tile
   if (c.offsets) {
-    for (int e = tid; e < c.sets; e += kRThreads) bounds[e] = set_slots(c.offsets, e, c.slots);
-    __syncthreads();
+    load_bounds<kRThreads>(bounds, c.offsets, c.sets, c.slots, tid);
     if (warp == 0) prefix_sums(first, c.sets, lane, [&](int e) { return (bounds[e].y - bounds[e].x + NT - 1) / NT * p.row_tiles; });
   } else if (tid == 0) {
     bounds[0] = make_int2(0, c.slots);

@@ -65,10 +65,25 @@ __device__ __forceinline__ float activate(float v, int act) {
 __device__ __forceinline__ int bias_index(int row, int N, int act) {
   return act == W4A16_ACT_SWIGLU ? (row >> 1) + (row & 1) * (N >> 1) : row;
 }
-// The set's slots, whatever the offsets hold: within [0, slots], the end not before the beginning.
-__device__ __forceinline__ int2 set_slots(const int32_t* offsets, int e, int slots) {
-  const int lo = min(max(__ldcg(offsets + e), 0), slots);
-  return make_int2(lo, min(max(__ldcg(offsets + e + 1), lo), slots));
+// The sets' slots into bounds[0 .. sets), by all THREADS threads of the block: within [0, slots] whatever the offsets hold, and no slot in two
+// sets. That keeps the number of units within what the launch was laid out for and no output is written twice. Offsets that descend somewhere
+// count as the largest before them; only then one thread goes through the sets again.
+template <int THREADS>
+__device__ __forceinline__ void load_bounds(int2* bounds, const int32_t* offsets, int sets, int slots, int tid) {
+  bool descend = false;
+  for (int e = tid; e < sets; e += THREADS) {
+    const int lo = min(max(__ldcg(offsets + e), 0), slots), hi = min(max(__ldcg(offsets + e + 1), 0), slots);
+    bounds[e] = make_int2(lo, hi);
+    descend |= hi < lo;
+  }
+  if (!__syncthreads_or(descend)) return;
+  if (tid == 0)
+    for (int e = 0, most = 0; e < sets; ++e) {
+      const int lo = max(most, bounds[e].x);
+      most = max(lo, bounds[e].y);
+      bounds[e] = make_int2(lo, most);
+    }
+  __syncthreads();
 }
 // Prefix sums of value(0 .. n - 1) into first[0 .. n], the sum in first[n], by one whole warp: a lane takes neighbours. (32 at a time with a
 // carry, 256 experts at one token 12.1 us instead of 11.7.)
