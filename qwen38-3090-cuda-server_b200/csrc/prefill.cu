@@ -902,12 +902,11 @@ PrefillPlan plan_prefill(int M, int pairs, int G, const int* device_clusters, in
 // The plan of a dense layer with an epilogue whose tokens fit one tile of a CTA alone: as many K splits as find clusters at
 // once. (row tiles of 128; clusters of S CTAs, as many at once as a B200 of 148 SMs runs)
 PrefillPlan plan_single(int M, int row_tiles, int G, const int* device_clusters, int smem_optin) {
-  constexpr int kClusters[kPMaxSplit + 1] = {0, 148, 74, 46, 33};
+  constexpr int kClusters[kPMaxSplit + 1] = {0, 148, 74, 45, 33};
   PrefillPlan plan;
   plan.pair = false;
   plan.tn = (M + 15) & ~15;
-  for (int S = 2; S <= kPMaxSplit && S <= G; ++S)
-    if (row_tiles <= kClusters[S] && row_tiles <= device_clusters[S]) plan.splits = S;
+  plan.splits = splits_at_once(row_tiles, G < kPMaxSplit ? G : kPMaxSplit, kClusters, device_clusters);
   plan.full_tt = M / plan.tn;
   plan.tiles = row_tiles;
   plan.clusters = plan.splits > 1 || row_tiles < device_clusters[1] ? row_tiles : device_clusters[1];

@@ -472,12 +472,11 @@ int launch_ragged(RaggedParams& p, const DeviceInfo* di, int max_units, cudaStre
   const int smem = fixed + p.depth * stage_bytes<NT>();
   // Few units: as many CTAs share one as there are clusters for at once. (One more, and a last cluster starts when a first one ends:
   // 5120 x 6144 at M = 1, 40 units: six 9.2 us, seven - of which 37 fit - 13.7; 5120 x 17408 17.6 and 24.0.)
+  constexpr int kRoom[kRMaxSplit + 1] = {0, 296, 148, 93, 71, 56, 45, 37, 33};
   const int* fit = clusters_at_once<NT>(di);
   if (!fit) return W4A16_ECUDA;
-  const int slots = fit[1];
-  int S = 1;
-  for (int n = 2; n <= kRMaxSplit && n * kRGroups <= p.c.G; ++n)
-    if (max_units <= fit[n]) S = n;
+  const int slots = fit[1], most = p.c.G / kRGroups < kRMaxSplit ? p.c.G / kRGroups : kRMaxSplit;
+  const int S = splits_at_once(max_units, most, kRoom, fit);
   p.splits = S;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute at[2];

@@ -121,6 +121,16 @@ __device__ __forceinline__ int set_of(int u, int e, const int* first, int sets) 
 }
 #endif
 
+// CTAs that share a tile's range of k: as many as there are clusters of for every tile at once. That goes by what a B200 of 148 SMs runs (`room`, by the
+// cluster's CTAs, as cudaOccupancyMaxActiveClusters answers there), not by what this device's GPCs happen to fit, so that a row has the same bits on
+// every GPU; the device's own answer (`runs`) only rules out clusters that it cannot run at all.
+inline int splits_at_once(int tiles, int most, const int* room, const int* runs) {
+  int splits = 1;
+  for (int n = 2; n <= most; ++n)
+    if (tiles <= room[n] && runs[n] >= 1) splits = n;
+  return splits;
+}
+
 inline bool ranges_apart(const void* a, size_t an, const void* b, size_t bn) {
   const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
   return x + an <= y || y + bn <= x;
