@@ -266,7 +266,8 @@ int w4a16_experts_linear(uint16_t* y, const w4a16_experts_t* w, const uint16_t* 
  *   offsets int32 [num_experts + 1]  first slot of every expert, then the number of slots
  *   rows    int32 [T * top_k] the token of every slot; entries behind the last slot stay as they were
  * (a logit of +inf counts as the largest finite one). Results are the same in every run. `workspace`: at least
- * w4a16_route_workspace(T, num_experts) bytes, 4-byte aligned, one call in flight per workspace. T = 0 writes the offsets. */
+ * w4a16_route_workspace(T, num_experts) bytes, 4-byte aligned, one call in flight per workspace. T = 0 writes the offsets.
+ * The five tables, the logits and the workspace must not overlap. */
 size_t w4a16_route_workspace(int max_tokens, int num_experts);
 int w4a16_route(int32_t* ids, float* weights, int32_t* offsets, int32_t* slots, int32_t* rows, const void* logits, int logits_are_f32,
                 int T, int num_experts, int top_k, int renormalize, void* workspace, size_t workspace_bytes, void* stream);

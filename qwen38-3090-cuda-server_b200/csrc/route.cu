@@ -431,6 +431,19 @@ int w4a16_route(int32_t* ids, float* weights, int32_t* offsets, int32_t* slots, 
   const int blocks = route_blocks(T);
   if (blocks > 1 && (workspace == nullptr || workspace_bytes < w4a16_route_workspace(T, num_experts)))
     return fail(W4A16_ESCRATCH, "route: workspace of %zu bytes for %d tokens, %zu needed", workspace_bytes, T, w4a16_route_workspace(T, num_experts));
+  // The second launch takes experts and counts as the first one left them, for indices: no table may lie in another, in the logits or in the workspace.
+  const size_t table = static_cast<size_t>(T) * top_k * 4;
+  const struct {
+    const void* at;
+    size_t bytes;
+  } written[] = {{ids, table}, {weights, table}, {slots, table}, {rows, table}, {offsets, (num_experts + 1) * sizeof(int32_t)},
+                 {blocks > 1 ? workspace : nullptr, blocks > 1 ? w4a16_route_workspace(T, num_experts) : 0}};
+  for (int i = 0; T > 0 && i < 6; ++i) {
+    W4_REQUIRE(ranges_apart(written[i].at, written[i].bytes, logits, static_cast<size_t>(T) * num_experts * (logits_are_f32 ? 4 : 2)),
+               "route: logits overlap a table or the workspace");
+    for (int j = 0; j < i; ++j)
+      W4_REQUIRE(ranges_apart(written[i].at, written[i].bytes, written[j].at, written[j].bytes), "route: a table overlaps another or the workspace");
+  }
   const DeviceInfo* di = device_info();
   if (!di) return W4A16_ECUDA;
   RouteParams p = {};
