@@ -212,8 +212,8 @@ __device__ __forceinline__ PTile tile_of(const PrefillParams& p, int tile) {
   return t;
 }
 
-// Sets: their slots and the tiles in front of each, in shared memory. A set's tokens are cut into equal tiles (a multiple of 32, at
-// most TN), which all expand the set's weights.
+// Sets: their slots and the tiles in front of each, in shared memory. A set's tokens are cut into equal tiles (a multiple of 32, for a CTA
+// alone of 16, and at most TN), which all expand the set's weights.
 struct SetTable {
   const int2* bounds;
   const int* first;  // [sets + 1]
@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(prefill_warps(MODE) * 32, 1) k_prefill(const _
       mbar_init(wempty_a + i * 8, 4);
     }
     for (int i = 0; i < kPDone; ++i) mbar_init(done_a + i * 8, 1);
-    // activations: one arrival that expects both CTAs' bytes; gathered rows: one arrival of each CTA
+    // activations: one arrival, the leader's, that expects the bytes of both CTAs (gathered rows: of all of the tile's tokens)
     for (int i = 0; i < kPSteps; ++i) mbar_init(xfull_a + i * 8, 1);
     for (int i = 0; i < kPMaxA; ++i) mbar_init(afull_a + i * 8, 4 * CG);
     mbar_init(dfull_a, 1);
@@ -465,9 +465,10 @@ __global__ void __launch_bounds__(prefill_warps(MODE) * 32, 1) k_prefill(const _
     // leader's barrier expects both CTAs' bytes.
     if (MODE == kSets && p.call.x_rows) {
       // Rows are gathered by TMA, four rows of 64 k a load, half of the tile's tokens in each CTA; places past the tile's tokens repeat
-      // the last one. Issuing a load takes a warp some 25 cycles and a group has up to 40, so three warps take the groups in turn, each with
-      // its own list of rows. 64 experts 2048 x 5120 of 8 picks, us at 300 / 1200 / 4096 tokens: one warp (a shuffle per row) 232 / 460 /
-      // 1270, two 178 / 319 / 831, with lists 145 / 267 / 675, three 140 / 245 / 623, four the same; rows already in slot order 133 / 216 / 548.
+      // the last one. Issuing a load takes a warp some 25 cycles and a group has up to 56 (28 fours of rows, two halves of the group's k), so
+      // three warps take the groups in turn, each with its own list of rows. 64 experts 2048 x 5120 of 8 picks, with tiles of 160 tokens (up to 40
+      // loads), us at 300 / 1200 / 4096 tokens: one warp (a shuffle per row) 232 / 460 / 1270, two 178 / 319 / 831, with lists 145 / 267 / 675,
+      // three 140 / 245 / 623, four the same; rows already in slot order 133 / 216 / 548.
       const uint32_t xfull_l = PAIR ? map_to_rank(xfull_a, leader) : xfull_a;
       int* rows = reinterpret_cast<int*>(bars + kPBars + 2) + (warp - kWActs) * (kPSetsTN / 2);  // (16-byte aligned)
       uint32_t j = 0;

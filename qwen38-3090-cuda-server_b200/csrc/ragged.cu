@@ -14,9 +14,10 @@
 //     expansion. The fragments' k order is free as long as both operands share it, so a lane takes 16 consecutive k of
 //     its row (8 bytes of codes) and of its token (two 16-byte loads). Two warps share 32 rows and add up their halves of K.
 //
-// What bounds it: the expansion's instructions. Two CTAs of an SM take some 500 cycles for a weight block where HBM allows 370: 1460
-// warp instructions at M = 8, of which LOP3, shifts and packed bf16 arithmetic issue at half a scheduler's rate (measured by themselves: 345 cycles without
-// the mma.sync, 408 with). 34816 x 5120 at M = 8 24.8 us (3.7 TB/s), 64 experts 5120 x 1024 at 4.1 slots each 52 (3.4 TB/s).
+// What bounds it: the expansion, and what its warps wait for in between. Two CTAs of an SM take 520 to 580 cycles for a weight block in long rows (and
+// 660 where a unit has eight blocks, its end among them), where HBM allows 370. Its 1310 warp instructions at M = 8, of which LOP3, shifts and packed bf16
+// arithmetic issue at half a scheduler's rate, take 345 cycles by themselves, 408 with the mma.sync; issue slots 56 to 60 % busy, no pipe above
+// 46 %. 34816 x 5120 at M = 8 24.2 us (3.8 TB/s), 64 experts 5120 x 1024 at 4.1 slots each 50.3 (3.5 TB/s), start and end of the launch included.
 // Tried beside it, the same or slower: 16 rows x 128 k per warp, three CTAs per SM, loads a step ahead, more accumulators, and A in tensor memory for
 // tcgen05.mma with two CTAs per SM (28.5 us at M = 1 against 25).
 #include <climits>
@@ -243,7 +244,7 @@ __global__ void __launch_bounds__(kRThreads, 2) k_ragged(const __grid_constant__
   if (warp == kRCons + 1) {
     // ================================================================ the rows' constants
     // All lanes of a row need the same ones: made once, read by one 16-byte load in place of eight small loads and eight permutes per lane
-    // and group (1460 instructions per weight block instead of 1630, 34816 x 5120 at M = 9).
+    // and group (170 of 1630 warp instructions per weight block, two chunks of tokens).
     uint32_t ph = 0;
     for (int u = cluster; !dead && u < units; u += nclusters) {
       for (int g = g0; g < g1; g += kRGroups) {

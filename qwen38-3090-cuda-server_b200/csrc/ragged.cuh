@@ -27,12 +27,14 @@ int launch_prefill_ragged(const RaggedCall& c, cudaStream_t stream);
 
 #ifdef __CUDACC__
 // v / (1 + exp(-v)); the gated and the tanh form come back to it: 0.5 v (1 + tanh u) = v / (1 + exp(-2 u)) holds its precision where
-// the tanh is near -1. Two special-function instructions a value.
+// the tanh is near -1. Two special-function instructions a value. From exp(-u) = 2^126 on (u = -87.3, results under 2^-119) the quotient is zero.
 __device__ __forceinline__ float logistic_times(float v, float u) { return __fdividef(v, 1.f + __expf(-u)); }
 
-// v / 2 erfc(-v / sqrt 2). With x = |v| / sqrt 2 and t = 1 / (1 + x / 2), erfc(x) = t exp(P(t) - x^2); P is the polynomial through ln(erfc(x)
-// exp(x^2) / t) at Chebyshev nodes of t for x in [0, 13.3], where erfc leaves fp32. Relative error of erfc 8e-7, in fp32 2e-6 for x < 4
-// and 8e-6 at the far end (2^-17, the rounding of x^2). (erfcf, a call of some 60 instructions per value, made 34816 x 5120 at M = 4096 with GELU
+// v / 2 erfc(-v / sqrt 2). With x = |v| / sqrt 2 and t = 1 / (1 + x / 2), erfc(x) = t exp(P(t) - x^2), the form of Numerical Recipes; P is a fit of our
+// own, the polynomial through ln(erfc(x) exp(x^2) / t) at Chebyshev nodes of t for x in [0, 13.3] (erfc leaves fp32 at x = 10). Relative error
+// of erfc by the polynomial 8e-7; with the steps in fp32 (x^2 counts the rounding of x twice) 2.2e-6 for x < 4, 7.6e-6 at x = 7.7 (v = -10.8), 1.7e-5
+// at x = 10, the last emulated with an exact exp, to which __expf adds up to (2 + 1.2 x^2) 2^-23: 2^-15.8 in all where the result is above
+// 2^-92, 2^-15 where erfc leaves fp32; rounding to bf16 adds 2^-8. (erfcf, a call of some 60 instructions per value, made 34816 x 5120 at M = 4096 with GELU
 // 1437 us instead of 1235.)
 __device__ __forceinline__ float gelu_erf(float v) {
   const float x = 0.70710678119f * fabsf(v), t = __fdividef(1.f, 1.f + 0.5f * x);

@@ -58,8 +58,8 @@ __device__ __forceinline__ void scan_experts(int* totals, int E, int lane) {
 // largest key over the warp, then the lowest index that has it. Within a block the tokens that picked an expert are the bits of a
 // word, so that a pick's place among them is a population count: sorted by expert and token without sorting.
 // With one block the slots follow at once; otherwise the block's counts go out and k_route_scan and k_route_slots finish.
-// Bound by its launches and their dependences: one token of 64 experts 5.7 us as an eager call, nearly all the host's (3.2 in a graph), 4096 tokens of 256
-// experts 15.7 us in three launches, where the logits take 0.7 at HBM's rate. Counts added up by one CTA 28 us, by every block for itself 21.9.
+// Bound by its launches and their dependences: one token of 64 experts 5.8 us as an eager call, nearly all the host's (2.8 in a graph), 4096 tokens of 256
+// experts 15.6 us in three launches (15.1 in a graph, 16.9 with the logits in HBM), where the logits take 0.7 at HBM's rate.
 template <int EPL, int PER>
 __global__ void __launch_bounds__(PER * 32) k_route(const RouteParams p) {
   __shared__ uint32_t masks[kMaxSets];
@@ -463,7 +463,9 @@ int w4a16_route(int32_t* ids, float* weights, int32_t* offsets, int32_t* slots, 
   // as their counts fit the workspace. Counts of few blocks are added up by every block of k_route_slots, of more by a kernel in between.
   // us in a graph, blocks of 32 and the kernel in between / this: 64 experts, 33 tokens 7.0 / 4.7, 1000 8.1 / 6.7; 256: 10.2 / 7.1,
   // 12.0 / 11.6; 512: 14.3 / 9.9, 18 / 15.7.
-  // Adding up 16384 words (512 experts, 4096 tokens) 23.6, the kernel in between 22.2.
+  // Without eight tokens to a block, the kernel in between / adding up: 64 experts, 4000 tokens (2000 words) 11.4 / 10.1; 128, 8000 (8000) 14.4 / 13.6, 8192
+  // (8192) 13.1 / 13.7; 256, 2000 (4032) 13.9 / 14.0, 4000 (8000) 15.0 / 15.2, 4096 (8192) 15.1 / 15.3, 8192 (16384) 15.6 / 18.2; 512, 1300 (5248)
+  // 17.4 / 20.6, 2048 (8192) 19.7 / 22.1, 4096 (16384) 23.5 / 26.0. Around 8000 words it is even, but for 512 experts, which would want fewer.
   const long long row_words = (num_experts + 3) / 4, narrow = (static_cast<long long>(T) + kRouteFewWarps - 1) / kRouteFewWarps;
   const bool spread = blocks > 1 && T <= kRouteFewWarps * di->sms && narrow * row_words <= kRouteFewWords &&
                       narrow * row_words <= (blocks + 1LL) * num_experts;
