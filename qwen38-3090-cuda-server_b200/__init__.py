@@ -476,6 +476,7 @@ class Route:
             starts.append(starts[-1] + (n + 3) // 4 * 4)
         self._memory = torch.zeros(starts[-1], dtype=torch.int32, device="cuda")
         self._starts, self._at, self._pointers = starts[:-1], None, []
+        self._device = self._memory.get_device()
         ids, weights, offsets, slots, rows = (self._memory[at:at + n] for at, n in zip(starts, sizes))
         self.ids, self.slots = ids.view(max_tokens, top_k), slots.view(max_tokens, top_k)
         self.weights = weights.view(torch.float32).view(max_tokens, top_k)
@@ -504,6 +505,8 @@ def route(r: Route, logits, renormalize: bool = True, stream=None):
     if T > r.max_tokens:
         raise W4A16Error(-1, f"route: {T} tokens, room for {r.max_tokens}")
     dev, f32 = _device(), logits.dtype is _F32
+    if dev != r._device:
+        raise W4A16Error(-1, f"route: the tables are on device {r._device}, the current one is {dev}")
     _want("route: logits", logits, _F32 if f32 else _BF16, T * r.num_experts, dev)
     _want("route: workspace", r.workspace, _I32, r.workspace_bytes // 4, dev)
     memory = r._memory.data_ptr()

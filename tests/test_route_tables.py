@@ -94,6 +94,17 @@ def test_a_table_with_other_memory_leaves_the_calls_where_they_were(pkg, route):
         assert all(lo <= address and address + 4 * n <= lo + size for address, n in zip(calls[-1], (15, 15, 8, 15, 15)))
 
 
+def test_another_device_is_refused(pkg, route, monkeypatch):
+    """Whatever logits and workspace are handed over there."""
+    make, calls = route
+    r = make(5, 7, 3)
+    monkeypatch.setattr(pkg, "_device", lambda: 1)
+    monkeypatch.setattr(pkg, "_want", lambda *a: None)
+    with pytest.raises(pkg.W4A16Error) as e:
+        pkg.route(r, torch.zeros((5, 7)))
+    assert "device" in str(e.value) and not calls
+
+
 def test_copies_have_memory_of_their_own(pkg, route):
     make, calls = route
     r = make(5, 7, 3)
